@@ -75,7 +75,9 @@ const char *mllb_last_error(void);
  * of range; bit 4 = decode position outside the KV cache; bit 5 = decode
  * attention gave up waiting for its K/V copies; bit 6 = a peer all-gather
  * gave up waiting for another rank; bit 7 = a grid-wide epilogue
- * (mllb_q4k_matvec_norm) gave up waiting for the other CTAs of its grid.
+ * (mllb_q4k_matvec_norm) gave up waiting for the other CTAs of its grid;
+ * bit 8 = a page, sequence or length of a paged cache outside its table or
+ * cache; bit 9 = a beam's parent outside its batch entry.
  * Copies the word of the current device to *bits (synchronising),
  * optionally clearing it.  0 in normal runs.
  */
@@ -507,6 +509,139 @@ int mllb_decode_attention_qkv_q4_0(const float *qkv, const float *q_gamma, const
  * (integration/logit_validation.h:76-80).
  */
 int mllb_argmax_f32(const float *x, int64_t n, int64_t index_offset, int64_t *key, unsigned flags, void *stream);
+
+/* ------------------------------------------------------------------------
+ * Many sequences over a KV cache in pages: the append with norms and rotary
+ * positions, attention over prefixes that sequences share and over their own
+ * rows, and beam search's selection and reordering.  Table entries, lengths
+ * and rows are read on the device (a captured graph follows them); one that
+ * lies outside its table or cache sets device error bit 8 (mask 0x100) and
+ * reads or writes nothing through it.
+ * ---------------------------------------------------------------------- */
+
+#define MLLB_TYPE_F32 0
+#define MLLB_TYPE_F16 1
+#define MLLB_TYPE_BF16 2
+
+/*
+ * Pages of page_size rows (a power of two, 16 to 1024) for each of kv_heads
+ * heads, K and V apart, fp16 or bf16.  Element (page, head, row, e) is at
+ * page * page_stride + head * head_stride + row * row_stride + e (strides in
+ * elements, multiples of 8, the same for K and V), so heads may lie ahead of
+ * rows in a page or behind them.  head_dim 64 or 128.  layers, layer_stride:
+ * several layers' caches with one page numbering (mllb_beam_reorder); 1 and
+ * ignored elsewhere.  Row r of a sequence is row r % page_size of page
+ * table[r / page_size] of its line in a page table.
+ */
+typedef struct mllb_paged_cache {
+    void *k, *v;
+    int64_t pages, kv_heads, page_size, head_dim;
+    int64_t page_stride, head_stride, row_stride;
+    int64_t layers, layer_stride;
+    int32_t type; /* MLLB_TYPE_F16 or MLLB_TYPE_BF16 */
+} mllb_paged_cache;
+
+/*
+ * For each token t (qkv row t: q heads, k heads, v heads of head_dim values):
+ *   q, k heads: x / sqrt(mean(x^2) + eps) * gamma (skipped where the gamma is
+ *     NULL), then the first rot_dim elements turn by positions[t] * freqs[i]
+ *     radians, pairs (i, i + rot_dim / 2), or (2i, 2i + 1) if interleaved,
+ *     and are multiplied by magnitude;
+ *   q -> q_out [tokens][q_heads][head_dim] (the cache's type), k and v -> row
+ *   rows[t] of sequence seq[t] (seq NULL: of sequence t).
+ * A negative rows[t] is padding: nothing is stored for it, q_out neither.  A
+ * row without a page stores q_out only (and sets bit 8).  No (sequence, row)
+ * may come twice in a call.  fp32 arithmetic, fp64 angles.
+ */
+typedef struct mllb_paged_append {
+    const void *qkv;
+    int64_t tokens, qkv_stride; /* stride of a token in elements; 16-byte multiples */
+    const int32_t *positions, *rows, *seq, *page_table;
+    int64_t seqs, table_width; /* page_table is [seqs][table_width] */
+    const float *q_gamma, *k_gamma;
+    const double *freqs; /* [rot_dim / 2] */
+    int64_t rot_dim, q_heads;
+    double eps, magnitude;
+    void *q_out;
+    int32_t qkv_type, interleaved;
+} mllb_paged_append;
+int mllb_paged_qkv_append(const mllb_paged_append *args, const mllb_paged_cache *cache, unsigned flags, void *stream);
+
+/*
+ * Attention of tokens over their group's prefix and their sequence's own rows:
+ *   out[t][h] = softmax over the visible j of (scale q[t][h] . k_j) applied to v_j
+ * Sequence b's tokens are q_start[b] .. q_start[b + 1] - 1 (q_start NULL: one
+ * each), its last ones: of n tokens, token i sees its own rows below
+ * seq_lens[b] - n + i + 1.  Sequences group_start[g] .. group_start[g + 1] - 1
+ * also see all prefix_lens[g] rows of prefix_table[g]; a group's prefix is
+ * read once for all its sequences where they have few tokens.  groups 0: no
+ * prefixes; group_start NULL: one group of all sequences.  A token that sees
+ * nothing gets zeros; tokens behind q_start[seqs] stay as they are.  Rows
+ * behind a sequence's length may hold anything, NaN too; the visible ones,
+ * and those of a sequence's later tokens, must be finite.  q head h reads KV
+ * head h / (q_heads / kv_heads).  q and out have the cache's type; fp32
+ * softmax and sums, the weights rounded to the cache's type for the products
+ * with V.  workspace: mllb_paged_attention_workspace bytes (the number
+ * depends on the current device), 16-byte aligned, any contents; calls that
+ * share it must not overlap on the GPU.  seqs + groups <= 2048.
+ */
+typedef struct mllb_paged_attn {
+    const void *q;
+    void *out;
+    int64_t tokens, q_heads;
+    int64_t q_token_stride, q_head_stride, out_token_stride, out_head_stride; /* elements, multiples of 8 */
+    const int32_t *page_table, *seq_lens; /* [seqs][table_width], [seqs] */
+    int64_t seqs, table_width;
+    const int32_t *prefix_table, *prefix_lens, *group_start; /* [groups][prefix_width], [groups], [groups + 1] */
+    int64_t groups, prefix_width;
+    const int32_t *q_start; /* [seqs + 1] or NULL */
+    double scale;
+} mllb_paged_attn;
+int64_t mllb_paged_attention_workspace(int64_t tokens, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
+                                       int64_t seqs, int64_t groups);
+int mllb_paged_attention(const mllb_paged_attn *args, const mllb_paged_cache *cache, void *workspace,
+                         int64_t workspace_bytes, unsigned flags, void *stream);
+
+/*
+ * The n best continuations of each batch entry over beams x vocabulary:
+ *   score[w][v] = scores[w] + logits[w][v] - log(sum_u exp(logits[w][u]))
+ * in descending order, ties to the lower beam, in it to the larger logit, then
+ * to the lower token -> out_scores, out_tokens (v), out_parents (w),
+ * [batch][n] each.  NaN logits count as
+ * -inf, +inf as the largest finite fp32.  A logit of -inf is no candidate;
+ * a done beam's only candidate is end_token at the beam's score.  Places
+ * without a candidate: -inf, -1, -1.  beams and n at most 64, vocab at most
+ * 2^26.  Scores are compared in fp64.  workspace as for the attention.
+ */
+typedef struct mllb_beam_scores {
+    const void *logits; /* [batch][beams][vocab], strides in elements */
+    int64_t batch, beams, vocab, n, batch_stride, beam_stride;
+    const float *scores;  /* [batch][beams] */
+    const uint8_t *done;  /* [batch][beams] or NULL */
+    int64_t end_token;    /* used with done */
+    int32_t type;         /* MLLB_TYPE_* of the logits */
+} mllb_beam_scores;
+int64_t mllb_beam_select_workspace(int64_t batch, int64_t beams, int64_t vocab, int64_t n);
+int mllb_beam_select(const mllb_beam_scores *args, float *out_scores, int32_t *out_tokens, int32_t *out_parents,
+                     void *workspace, int64_t workspace_bytes, unsigned flags, void *stream);
+
+/*
+ * Row r = (entry, beam) of the page table and lengths becomes its parent's
+ * (parents[r]: a beam of the same entry).  Whole pages are shared; the last,
+ * part-full page goes on being written, so the first child of a parent (the
+ * lowest r) keeps it and every other child gets fresh[r] in its place, with
+ * the rows held copied for K and V of all layers; used[r] = 1 where fresh[r]
+ * was taken.  fresh: distinct pages that no table line names.  A negative
+ * parent ends the row (length 0, table -1), one past the beams also sets
+ * device error bit 9 (mask 0x200).  table_out and lens_out must not overlap
+ * the inputs.
+ */
+typedef struct mllb_beam_rows {
+    const int32_t *parents, *page_table, *seq_lens, *fresh;
+    int64_t batch, beams, table_width;
+} mllb_beam_rows;
+int mllb_beam_reorder(const mllb_beam_rows *args, const mllb_paged_cache *cache, int32_t *table_out, int32_t *lens_out,
+                      int32_t *used, unsigned flags, void *stream);
 
 #ifdef __cplusplus
 }

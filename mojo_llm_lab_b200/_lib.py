@@ -21,6 +21,10 @@ MLLB_EALIGN = -2
 MLLB_ECUDA = -3
 MLLB_EUNSUPPORTED = -4
 
+TYPE_F32 = 0
+TYPE_F16 = 1
+TYPE_BF16 = 2
+
 LAUNCH_PDL = 1
 LAUNCH_CONST_AUX = 2  # IMROPE: gamma / positions / theta not written by the preceding kernel
 
@@ -45,6 +49,42 @@ class PeerGather(C.Structure):
     """mllb_peer_gather of include/mllb200.h."""
     _fields_ = [("rank", C.c_int32), ("world", C.c_int32), ("buffers", C.c_void_p * 8),
                 ("flags", C.c_void_p * 8), ("count", C.c_void_p)]
+
+
+class PagedCache(C.Structure):
+    """mllb_paged_cache of include/mllb200.h."""
+    _fields_ = [("k", _P), ("v", _P), ("pages", _I64), ("kv_heads", _I64), ("page_size", _I64), ("head_dim", _I64),
+                ("page_stride", _I64), ("head_stride", _I64), ("row_stride", _I64), ("layers", _I64),
+                ("layer_stride", _I64), ("type", C.c_int32)]
+
+
+class PagedAppend(C.Structure):
+    """mllb_paged_append of include/mllb200.h."""
+    _fields_ = [("qkv", _P), ("tokens", _I64), ("qkv_stride", _I64), ("positions", _P), ("rows", _P), ("seq", _P),
+                ("page_table", _P), ("seqs", _I64), ("table_width", _I64), ("q_gamma", _P), ("k_gamma", _P),
+                ("freqs", _P), ("rot_dim", _I64), ("q_heads", _I64), ("eps", C.c_double), ("magnitude", C.c_double),
+                ("q_out", _P), ("qkv_type", C.c_int32), ("interleaved", C.c_int32)]
+
+
+class PagedAttn(C.Structure):
+    """mllb_paged_attn of include/mllb200.h."""
+    _fields_ = [("q", _P), ("out", _P), ("tokens", _I64), ("q_heads", _I64), ("q_token_stride", _I64),
+                ("q_head_stride", _I64), ("out_token_stride", _I64), ("out_head_stride", _I64), ("page_table", _P),
+                ("seq_lens", _P), ("seqs", _I64), ("table_width", _I64), ("prefix_table", _P), ("prefix_lens", _P),
+                ("group_start", _P), ("groups", _I64), ("prefix_width", _I64), ("q_start", _P), ("scale", C.c_double)]
+
+
+class BeamScores(C.Structure):
+    """mllb_beam_scores of include/mllb200.h."""
+    _fields_ = [("logits", _P), ("batch", _I64), ("beams", _I64), ("vocab", _I64), ("n", _I64), ("batch_stride", _I64),
+                ("beam_stride", _I64), ("scores", _P), ("done", _P), ("end_token", _I64), ("type", C.c_int32)]
+
+
+class BeamRows(C.Structure):
+    """mllb_beam_rows of include/mllb200.h."""
+    _fields_ = [("parents", _P), ("page_table", _P), ("seq_lens", _P), ("fresh", _P), ("batch", _I64), ("beams", _I64),
+                ("table_width", _I64)]
+
 
 SIGNATURES = {
     "mllb_abi_version": (C.c_int, []),
@@ -95,6 +135,12 @@ SIGNATURES = {
     "mllb_q4k_matvec_norm": (C.c_int, [_P, _P, _P, _I64, _I64, _P, _P, _P, C.c_double, _P, _P, _I64, C.c_uint, _P]),
     "mllb_q4k_matmul_tokens_workspace": (C.c_int64, [_I64, _I64, _I64]),
     "mllb_q4k_matmul_tokens": (C.c_int, [_P, _P, _P, _I64, _I64, _I64, _P, _I64, C.c_uint, _P]),
+    "mllb_paged_qkv_append": (C.c_int, [C.POINTER(PagedAppend), C.POINTER(PagedCache), C.c_uint, _P]),
+    "mllb_paged_attention_workspace": (_I64, [_I64, _I64, _I64, _I64, _I64, _I64]),
+    "mllb_paged_attention": (C.c_int, [C.POINTER(PagedAttn), C.POINTER(PagedCache), _P, _I64, C.c_uint, _P]),
+    "mllb_beam_select_workspace": (_I64, [_I64, _I64, _I64, _I64]),
+    "mllb_beam_select": (C.c_int, [C.POINTER(BeamScores), _P, _P, _P, _P, _I64, C.c_uint, _P]),
+    "mllb_beam_reorder": (C.c_int, [C.POINTER(BeamRows), C.POINTER(PagedCache), _P, _P, _P, C.c_uint, _P]),
 }
 
 _lock = threading.Lock()

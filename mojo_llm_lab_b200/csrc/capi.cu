@@ -1352,3 +1352,5 @@ extern "C" int mllb_q5k_matvec_ex(const void* weights, const void* q8, float* ou
 extern "C" int mllb_q5k_matvec(const void* weights, const void* q8, float* out, int64_t n, int64_t k, void* stream) {
   return mllb_q5k_matvec_ex(weights, q8, out, n, k, 0u, stream);
 }
+
+#include "paged_capi.cuh"

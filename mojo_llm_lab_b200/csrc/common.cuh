@@ -26,6 +26,8 @@ enum : uint32_t {
   kErrKvWaitTimeout = 1u << 5,     // decode attention gave up waiting for its K/V copies
   kErrPeerWaitTimeout = 1u << 6,   // peer all-gather gave up waiting for another rank's slice
   kErrGridWaitTimeout = 1u << 7,   // a grid-wide epilogue gave up waiting for the grid's other CTAs
+  kErrBadPage = 1u << 8,           // paged cache: a page, sequence or length outside the table or the cache
+  kErrBadParent = 1u << 9,         // beam reorder: a parent outside the batch entry (the row ends)
 };
 
 // Device-resident state of a decode loop; mirrors mllb_decode_state of the

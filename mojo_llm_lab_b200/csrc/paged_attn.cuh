@@ -1,0 +1,762 @@
+// Attention of a batch of sequences over a paged cache, with prefixes that
+// several sequences share.
+//
+//   out[t][h] = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale q . k_j - max)
+//
+// over the prefix of the token's group and the sequence's own rows up to the
+// token's.  Work comes as entities: a sequence (its own rows, or its prefix
+// and its own rows), or a group (its prefix under the queries of ALL its
+// sequences, so that the prefix is read once).  An entity's query rows are
+// (token, query head of a KV head), cut into tiles of R rows; a (row tile, KV
+// head) is an item, and its keys are cut into tiles of KT.  The (item, key
+// tile) pairs of all entities, in order, are one line that is cut into equal
+// shares, one per CTA, whatever the lengths: no CTA idles because one context
+// is long, and short ones are not padded.  The lengths are read on the device
+// (each CTA adds them up for itself), so a captured graph stays right while
+// they grow.
+//
+// A CTA's share of an item is a segment.  An item with one segment and
+// nothing else to add is written to out at once; otherwise segments leave
+// (maximum, sum, unnormalised accumulator) in fp32 in the workspace, and
+// paged_merge_kernel joins a row's segments.
+#pragma once
+
+#include <cuda.h>
+
+#include "paged.cuh"
+
+namespace mllb {
+
+enum : int {
+  kAttnOwn = 0,     // entities: sequences, own rows only
+  kAttnConcat = 1,  // entities: sequences, prefix then own rows
+  kAttnBoth = 2,    // entities: groups' prefixes, then sequences' own rows
+  kAttnPrefix = 3,  // entities: groups' prefixes
+};
+
+constexpr int kAttnMaxEntities = 2048;
+
+struct AttnArgs {
+  const uint16_t* q;  // [tokens][q_heads][D], strides in elements
+  uint16_t* out;
+  long long q_token, q_head, out_token, out_head;
+  const int32_t* table;         // [seqs][width]
+  const int32_t* lens;          // [seqs]
+  const int32_t* prefix_table;  // [groups][prefix_width]
+  const int32_t* prefix_lens;   // [groups]
+  const int32_t* group_start;   // [groups + 1], nullptr: one group of all sequences
+  const int32_t* q_start;       // [seqs + 1], nullptr: token b is sequence b's
+  int width, prefix_width, seqs, groups, tokens, kv_heads, ratio, page_shift, pages;
+  float scale_log2;  // scale x log2(e): the softmax runs on powers of two
+};
+
+// One launch's line of work and where its segments go.
+struct AttnPass {
+  int mode, entities, ctas;
+  int dense;       // 1: segment of CTA c and item i at slot c + i; 0: at 2 c (a CTA's first) or 2 c + 1
+  int slots;       // capacity of the workspace
+  int rows, keys;  // R and KT of the kernel that ran it (for the merge)
+  int32_t* plan;   // [2][entities + 1]: key tiles and items before each entity (for the merge)
+  float* acc;      // [slots][R][D]
+  float2* stats;   // [slots][R] (maximum in powers of two, sum)
+};
+
+struct AttnEntity {
+  int tok0, ntok, plen, len, causal;
+  const int32_t* ptab;
+  const int32_t* tab;
+};
+
+__device__ __forceinline__ int attn_clamp_len(int len, int width, int page_shift) {
+  const int most = width << page_shift;
+  if (len < 0 || len > most) record_error(kErrBadPage);
+  return min(max(len, 0), most);
+}
+
+__device__ __forceinline__ int attn_token_start(const AttnArgs& a, int seq) {
+  if (!a.q_start) return min(max(seq, 0), a.tokens);
+  return min(max(a.q_start[min(max(seq, 0), a.seqs)], 0), a.tokens);
+}
+
+// The group of a sequence, -1 if it has none.
+__device__ __forceinline__ int attn_group_of(const AttnArgs& a, int seq) {
+  if (a.groups == 0) return -1;
+  if (!a.group_start) return 0;
+  int lo = 0, hi = a.groups;  // group_start[lo] <= seq < group_start[hi], if any
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (a.group_start[mid] <= seq) lo = mid; else hi = mid;
+  }
+  return a.group_start[lo] <= seq && seq < a.group_start[lo + 1] ? lo : -1;
+}
+
+__device__ __forceinline__ AttnEntity attn_entity(const AttnArgs& a, int mode, int e) {
+  AttnEntity n;
+  n.plen = 0;
+  n.ptab = nullptr;
+  if (mode == kAttnPrefix || (mode == kAttnBoth && e < a.groups)) {
+    const int s0 = a.group_start ? a.group_start[e] : 0, s1 = a.group_start ? a.group_start[e + 1] : a.seqs;
+    n.tok0 = attn_token_start(a, s0);
+    n.ntok = max(attn_token_start(a, s1) - n.tok0, 0);
+    n.len = attn_clamp_len(a.prefix_lens[e], a.prefix_width, a.page_shift);
+    n.tab = a.prefix_table + static_cast<long long>(e) * a.prefix_width;
+    n.causal = 0;
+    return n;
+  }
+  const int seq = mode == kAttnBoth ? e - a.groups : e;
+  n.tok0 = attn_token_start(a, seq);
+  n.ntok = max(attn_token_start(a, seq + 1) - n.tok0, 0);
+  n.len = attn_clamp_len(a.lens[seq], a.width, a.page_shift);
+  n.tab = a.table + static_cast<long long>(seq) * a.width;
+  n.causal = 1;
+  if (mode == kAttnConcat) {
+    const int g = attn_group_of(a, seq);
+    if (g >= 0) {
+      n.plen = attn_clamp_len(a.prefix_lens[g], a.prefix_width, a.page_shift);
+      n.ptab = a.prefix_table + static_cast<long long>(g) * a.prefix_width;
+    }
+  }
+  return n;
+}
+
+// Own rows that the entity's token j sees.
+__device__ __forceinline__ int attn_limit(const AttnEntity& n, int j) {
+  return n.causal ? min(max(n.len - n.ntok + j + 1, 0), n.len) : n.len;
+}
+
+__device__ __forceinline__ int attn_row_tiles(const AttnEntity& n, int ratio, int R) {
+  return (n.ntok * ratio + R - 1) / R;
+}
+
+// Key tiles of row tile t: the prefix's, then the own rows' up to the last token's limit.
+__device__ __forceinline__ int attn_key_tiles(const AttnEntity& n, int ratio, int t, int R, int KT) {
+  const int last = min(n.ntok * ratio, (t + 1) * R) - 1;
+  return (n.plen + KT - 1) / KT + (attn_limit(n, last / ratio) + KT - 1) / KT;
+}
+
+// First pair of CTA c's share.  No more CTAs take part than there are pairs,
+// so every one of an item's CTAs, first to last, has a segment of it.
+__device__ __forceinline__ int attn_share(int total, int ctas, int c) {
+  return static_cast<int>(static_cast<long long>(total) * c / ctas);
+}
+
+// Where a CTA's share starts, and how far it goes.
+struct AttnCursor {
+  int left;        // key tiles left in the share
+  int e, t, h;     // entity, row tile, KV head
+  int begin;       // first key tile of the segment
+  int item;        // number of the item on the line
+};
+
+// Adds up all entities' work and finds this CTA's share.  All threads of the
+// CTA call it; `scan` is shared scratch of 2 (entities + 1) + 64 ints.  CTA 0
+// also leaves the sums in pass.plan.
+template <int R, int KT, int kThreads>
+__device__ __forceinline__ AttnCursor attn_start(const AttnArgs& a, const AttnPass& pass, int* scan) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  constexpr int kWarps = kThreads / 32;
+  int* tiles = scan;
+  int* items = scan + pass.entities + 1;
+  int* part = items + pass.entities + 1;  // [2][kWarps]
+  int tiles_before = 0, items_before = 0;
+  for (int e0 = 0; e0 < pass.entities; e0 += kThreads) {
+    int w = 0, n = 0;
+    if (e0 + tid < pass.entities) {
+      const AttnEntity ent = attn_entity(a, pass.mode, e0 + tid);
+      const int t = attn_row_tiles(ent, a.ratio, R);
+      if (t > 0) {
+        if (ent.causal && ent.ntok > 1)
+          for (int i = 0; i < t; ++i) w += attn_key_tiles(ent, a.ratio, i, R, KT);
+        else
+          w = t * attn_key_tiles(ent, a.ratio, 0, R, KT);
+      }
+      w *= a.kv_heads;
+      n = t * a.kv_heads;
+    }
+    int ws = w, ns = n;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int wu = __shfl_up_sync(0xffffffffu, ws, d), nu = __shfl_up_sync(0xffffffffu, ns, d);
+      if (lane >= d) ws += wu, ns += nu;
+    }
+    if (lane == 31) part[warp] = ws, part[kWarps + warp] = ns;
+    __syncthreads();
+    int wb = tiles_before, nb = items_before;
+    for (int i = 0; i < kWarps; ++i) {
+      if (i < warp) wb += part[i], nb += part[kWarps + i];
+      tiles_before += part[i];
+      items_before += part[kWarps + i];
+    }
+    if (e0 + tid < pass.entities) {
+      tiles[e0 + tid] = wb + ws - w;
+      items[e0 + tid] = nb + ns - n;
+    }
+    __syncthreads();
+  }
+  if (tid == 0) {
+    tiles[pass.entities] = tiles_before;
+    items[pass.entities] = items_before;
+  }
+  __syncthreads();
+  if (blockIdx.x == 0)
+    for (int i = tid; i < 2 * (pass.entities + 1); i += kThreads) pass.plan[i] = scan[i];
+  AttnCursor c;
+  const int ctas = min(pass.ctas, tiles_before);
+  const int w0 = attn_share(tiles_before, max(ctas, 1), blockIdx.x);
+  c.left = static_cast<int>(blockIdx.x) < ctas ? attn_share(tiles_before, ctas, blockIdx.x + 1) - w0 : 0;
+  c.e = c.t = c.h = c.begin = c.item = 0;
+  if (c.left > 0) {
+    int lo = 0, hi = pass.entities;  // tiles[lo] <= w0 < tiles[hi]
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (tiles[mid] <= w0) lo = mid; else hi = mid;
+    }
+    c.e = lo;
+    const AttnEntity ent = attn_entity(a, pass.mode, lo);
+    int rest = w0 - tiles[lo], k = attn_key_tiles(ent, a.ratio, 0, R, KT);
+    if (ent.causal && ent.ntok > 1) {
+      while (rest >= a.kv_heads * k) {
+        rest -= a.kv_heads * k;
+        k = attn_key_tiles(ent, a.ratio, ++c.t, R, KT);
+      }
+    } else {
+      c.t = rest / (a.kv_heads * k);
+      rest -= c.t * a.kv_heads * k;
+    }
+    c.h = rest / k;
+    c.begin = rest - c.h * k;
+    c.item = items[lo] + c.t * a.kv_heads + c.h;
+  }
+  __syncthreads();
+  return c;
+}
+
+// The segments of a share, one after the other.
+struct AttnSegment {
+  AttnEntity ent;
+  int t, h, begin, end;  // row tile, KV head, key tiles [begin, end) of `of`
+  int of, item;
+};
+
+template <int R, int KT>
+struct AttnWalk {
+  const AttnArgs& a;
+  int mode, entities;
+  AttnCursor c;
+  AttnEntity ent;
+  __device__ AttnWalk(const AttnArgs& args, const AttnPass& pass, const AttnCursor& start)
+      : a(args), mode(pass.mode), entities(pass.entities), c(start) {
+    if (c.left > 0) ent = attn_entity(a, mode, c.e);
+  }
+  __device__ bool next(AttnSegment* s) {
+    if (c.left <= 0) return false;
+    int k = 0;
+    for (;;) {  // skip row tiles that see nothing and entities without rows
+      const int tiles = attn_row_tiles(ent, a.ratio, R);
+      if (c.t < tiles) {
+        k = attn_key_tiles(ent, a.ratio, c.t, R, KT);
+        if (k > 0) break;
+        ++c.t;
+        c.item += a.kv_heads;
+      } else {
+        if (++c.e >= entities) return false;
+        c.t = 0;
+        ent = attn_entity(a, mode, c.e);
+      }
+    }
+    s->ent = ent;
+    s->t = c.t;
+    s->h = c.h;
+    s->begin = c.begin;
+    s->end = min(k, c.begin + c.left);
+    s->of = k;
+    s->item = c.item;
+    c.left -= s->end - s->begin;
+    c.begin = 0;
+    ++c.item;
+    if (++c.h == a.kv_heads) c.h = 0, ++c.t;
+    return true;
+  }
+};
+
+// Key tile k of an entity: which table, its first row there, and how many rows that table's part has.
+struct AttnTile {
+  const int32_t* tab;
+  int row0, rows, own;
+};
+template <int KT>
+__device__ __forceinline__ AttnTile attn_tile(const AttnEntity& n, int k) {
+  const int before = (n.plen + KT - 1) / KT;
+  if (k < before) return {n.ptab, k * KT, n.plen, 0};
+  return {n.tab, (k - before) * KT, n.len, 1};
+}
+
+// The page of tile row `row` (a multiple of the page size or inside a page);
+// rows behind the end and bad entries give page number `pages`, which the
+// copies fill with zeros.
+__device__ __forceinline__ int attn_page(const AttnArgs& a, const AttnTile& tile, int row) {
+  const int r = tile.row0 + row;
+  if (r >= tile.rows) return a.pages;
+  const int page = tile.tab[r >> a.page_shift];
+  if (page >= 0 && page < a.pages) return page;
+  record_error(kErrBadPage);
+  return a.pages;
+}
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// TMA box (64 elements x box rows of one page and head) into a 128-byte-swizzled tile.
+__device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, int c0, int c1, int c2, int c3,
+                                            uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
+      "[%6];" ::"r"(smem_addr(dst)),
+      "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(smem_addr(bar))
+      : "memory");
+}
+__device__ __forceinline__ void tma_prefetch_map(const CUtensorMap* map) {
+  asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
+}
+
+__device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldsm4t(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+template <bool kBf16>
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (kBf16)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+                 "{%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+                 "{%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// ------------------------------------------------------------ few rows a key
+//
+// Row tiles of R = 16, 32 or 64: a key is used for at most R rows, so HBM
+// bounds it (2 R flops a byte; the warp-level matrix instructions do R = 64
+// in the time the tile takes to arrive) and what matters is copies in flight.
+// Four warps compute: R / 16 of them side by side over the rows, the rest
+// over the keys of a tile (each with its own maximum and sum, joined once per
+// segment through shared memory).  A fifth issues the copies: a ring of
+// three K + V tiles of 64 keys, so two CTAs per SM keep 100 KB or more in
+// flight.
+template <int D, int R>
+struct AttnFew {
+  static constexpr int kKeys = 64;
+  static constexpr int kStages = 3;
+  static constexpr int kThreads = 160;
+  static constexpr int kTile = kKeys * D * 2;            // bytes of a K or V tile
+  static constexpr int kStage = 2 * kTile;
+  static constexpr int kRowWarps = R / 16, kKeyWarps = 4 / kRowWarps, kWarpKeys = kKeys / kKeyWarps;
+  static constexpr int kJoin = 64 * D * 4 / 2;           // fp32 accumulators of two warps
+  static constexpr int kStatsOff = kStages * kStage + (kKeyWarps > 1 ? kJoin : 0);
+  static constexpr int kBarOff = kStatsOff + 4 * 16 * 8;
+  static constexpr int kSmem = kBarOff + 64;
+  static_assert(kStages * kStage >= (2 * (kAttnMaxEntities + 1) + 64) * 4, "the scan fits in the ring");
+};
+
+template <int D, int R, bool kBf16>
+__global__ void __launch_bounds__(160, 2)
+    paged_attn_few_kernel(const AttnArgs a, const AttnPass pass, const __grid_constant__ CUtensorMap kmap,
+                          const __grid_constant__ CUtensorMap vmap) {
+  using C = AttnFew<D, R>;
+  constexpr int KT = C::kKeys;
+  extern __shared__ __align__(1024) uint8_t attn_smem[];
+  uint8_t* ring = attn_smem;
+  float* join = reinterpret_cast<float*>(attn_smem + C::kStages * C::kStage);
+  float2* row_stats = reinterpret_cast<float2*>(attn_smem + C::kStatsOff);  // [4 warps][16]
+  uint64_t* full = reinterpret_cast<uint64_t*>(attn_smem + C::kBarOff);
+  uint64_t* empty = full + C::kStages;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < C::kStages; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 4);
+    }
+    fence_mbar_init();
+    tma_prefetch_map(&kmap);
+    tma_prefetch_map(&vmap);
+  }
+  pdl_wait_prerequisite();
+  pdl_launch_dependents();
+  const AttnCursor start = attn_start<R, KT, C::kThreads>(a, pass, reinterpret_cast<int*>(ring));
+  // The scan used the ring through the generic proxy; the copies come through the async one.
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  __syncthreads();
+  AttnWalk<R, KT> walk(a, pass, start);
+  AttnSegment s;
+
+  if (warp == 4) {
+    // ------------------------------------------------ copies
+    // Lanes take one box each: page p of the tile, half of the head, K or V.
+    const int box_rows = min(1 << a.page_shift, KT), per_tile = KT / box_rows;
+    constexpr int kHalves = D / 64;
+    const int boxes = per_tile * kHalves * 2;
+    int n = 0;
+    bool stuck = false;
+    while (!stuck && walk.next(&s)) {
+      for (int k = s.begin; k < s.end; ++k, ++n) {
+        const AttnTile tile = attn_tile<KT>(s.ent, k);
+        const int p = lane % per_tile, rest = lane / per_tile, half = rest % kHalves, is_v = rest / kHalves;
+        int page = 0;
+        if (lane < boxes) page = attn_page(a, tile, p * box_rows);
+        const int in_page = (tile.row0 + p * box_rows) & ((1 << a.page_shift) - 1);
+        const int st = n % C::kStages;
+        if (n >= C::kStages && !mbar_wait_bounded(&empty[st], (n / C::kStages - 1) & 1)) {
+          record_error(kErrEmptyWaitTimeout);
+          stuck = true;
+          break;
+        }
+        if (lane == 0) mbar_arrive_expect_tx(&full[st], C::kStage);
+        __syncwarp();
+        if (lane < boxes)
+          tma_load_4d(ring + st * C::kStage + is_v * C::kTile + half * (KT * 128) + p * box_rows * 128,
+                      is_v ? &vmap : &kmap, half * 64, in_page, s.h, page, &full[st]);
+      }
+    }
+    // The last copies land before the CTA's shared memory is given back.
+    for (int i = max(n - C::kStages, 0); i < n; ++i)
+      if (!mbar_wait_bounded(&full[i % C::kStages], (i / C::kStages) & 1)) record_error(kErrDrainTimeout);
+    return;
+  }
+
+  // -------------------------------------------------- products
+  const int rw = warp % C::kRowWarps, kw = warp / C::kRowWarps;
+  const int g = lane >> 2, tq = lane & 3;
+  int n = 0;
+  bool first = true, stuck = false;
+  while (walk.next(&s)) {
+    const int rows = s.ent.ntok * a.ratio;
+    int row[2], token[2], head[2], limit[2];
+    uint32_t q[D / 16][4];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      row[i] = s.t * R + rw * 16 + g + i * 8;
+      const bool there = row[i] < rows;
+      const int j = there ? row[i] / a.ratio : 0;
+      token[i] = there ? s.ent.tok0 + j : -1;
+      head[i] = s.h * a.ratio + (there ? row[i] - j * a.ratio : 0);
+      limit[i] = there ? attn_limit(s.ent, j) : 0;
+      const uint32_t* src = reinterpret_cast<const uint32_t*>(a.q + max(token[i], 0) * a.q_token + head[i] * a.q_head);
+#pragma unroll
+      for (int c = 0; c < D / 16; ++c) {
+        q[c][i] = there ? src[c * 8 + tq] : 0u;
+        q[c][i + 2] = there ? src[c * 8 + 4 + tq] : 0u;
+      }
+    }
+    float acc[D / 8][4];
+#pragma unroll
+    for (int i = 0; i < D / 8; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.0f;
+    float top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.0f, 0.0f};
+
+    for (int k = s.begin; k < s.end; ++k, ++n) {
+      const AttnTile tile = attn_tile<KT>(s.ent, k);
+      const int st = n % C::kStages;
+      if (!stuck && !mbar_wait_bounded(&full[st], (n / C::kStages) & 1)) {
+        record_error(kErrFullWaitTimeout);  // finish on what is there: the other warps wait at barriers
+        stuck = true;
+      }
+      const uint32_t kbase = smem_addr(ring + st * C::kStage), vbase = kbase + C::kTile;
+      constexpr int NT = C::kWarpKeys / 8;
+      const int key0 = kw * C::kWarpKeys;
+      float x[NT][4];
+#pragma unroll
+      for (int i = 0; i < NT; ++i) x[i][0] = x[i][1] = x[i][2] = x[i][3] = 0.0f;
+#pragma unroll
+      for (int c = 0; c < D / 16; ++c) {
+#pragma unroll
+        for (int i = 0; i < NT; i += 2) {
+          // Two 8-key blocks x two 8-element halves of the 16-element step.
+          const int r = key0 + i * 8 + (lane & 7) + ((lane >> 4) << 3);
+          const int chunk = c * 2 + ((lane >> 3) & 1);
+          uint32_t b[4];
+          ldsm4(kbase + (chunk >> 3) * (KT * 128) + r * 128 + (((chunk & 7) ^ (r & 7)) << 4), b);
+          mma16816<kBf16>(x[i], q[c], b[0], b[1]);
+          mma16816<kBf16>(x[i + 1], q[c], b[2], b[3]);
+        }
+      }
+      // Keys a row does not see weigh nothing, whatever their scores are.
+      const int end0 = min(tile.own ? limit[0] : tile.rows, tile.rows) - tile.row0;
+      const int end1 = min(tile.own ? limit[1] : tile.rows, tile.rows) - tile.row0;
+      float m0 = top[0], m1 = top[1];
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
+        const int key = key0 + i * 8 + tq * 2;
+        x[i][0] = key < end0 ? x[i][0] * a.scale_log2 : -INFINITY;
+        x[i][1] = key + 1 < end0 ? x[i][1] * a.scale_log2 : -INFINITY;
+        x[i][2] = key < end1 ? x[i][2] * a.scale_log2 : -INFINITY;
+        x[i][3] = key + 1 < end1 ? x[i][3] * a.scale_log2 : -INFINITY;
+        m0 = fmaxf(m0, fmaxf(x[i][0], x[i][1]));
+        m1 = fmaxf(m1, fmaxf(x[i][2], x[i][3]));
+      }
+#pragma unroll
+      for (int d = 1; d < 4; d <<= 1) {
+        m0 = fmaxf(m0, __shfl_xor_sync(0xffffffffu, m0, d));
+        m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, d));
+      }
+      const float z0 = m0 == -INFINITY ? 0.0f : m0, z1 = m1 == -INFINITY ? 0.0f : m1;
+      const float f0 = ex2(top[0] - z0), f1 = ex2(top[1] - z1);
+      top[0] = m0;
+      top[1] = m1;
+      sum[0] *= f0;
+      sum[1] *= f1;
+#pragma unroll
+      for (int i = 0; i < D / 8; ++i) {
+        acc[i][0] *= f0;
+        acc[i][1] *= f0;
+        acc[i][2] *= f1;
+        acc[i][3] *= f1;
+      }
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
+        x[i][0] = ex2(x[i][0] - z0);
+        x[i][1] = ex2(x[i][1] - z0);
+        x[i][2] = ex2(x[i][2] - z1);
+        x[i][3] = ex2(x[i][3] - z1);
+        sum[0] += x[i][0] + x[i][1];
+        sum[1] += x[i][2] + x[i][3];
+      }
+      // P in the cache's type (a factor 1 + 2^-11 or 2^-8 at most on each
+      // weight; the sums keep the unrounded ones).  V rows behind the end of
+      // a sequence are anything at all, NaN too: those registers become zero.
+      const int held = tile.rows - tile.row0;
+#pragma unroll
+      for (int i = 0; i < NT; i += 2) {
+        uint32_t p[4] = {pack16<kBf16>(x[i][0], x[i][1]), pack16<kBf16>(x[i][2], x[i][3]),
+                         pack16<kBf16>(x[i + 1][0], x[i + 1][1]), pack16<kBf16>(x[i + 1][2], x[i + 1][3])};
+        const int k0 = key0 + i * 8 + tq * 2;
+        const uint32_t lo = (k0 < held ? 0xffffu : 0u) | (k0 + 1 < held ? 0xffff0000u : 0u);
+        const uint32_t hi = (k0 + 8 < held ? 0xffffu : 0u) | (k0 + 9 < held ? 0xffff0000u : 0u);
+#pragma unroll
+        for (int c = 0; c < D / 8; c += 2) {
+          const int r = key0 + i * 8 + (lane & 15);
+          const int chunk = c + (lane >> 4);
+          uint32_t b[4];
+          ldsm4t(vbase + (chunk >> 3) * (KT * 128) + r * 128 + (((chunk & 7) ^ (r & 7)) << 4), b);
+          mma16816<kBf16>(acc[c], p, b[0] & lo, b[1] & hi);
+          mma16816<kBf16>(acc[c + 1], p, b[2] & lo, b[3] & hi);
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&empty[st]);
+    }
+#pragma unroll
+    for (int d = 1; d < 4; d <<= 1) {
+      sum[0] += __shfl_xor_sync(0xffffffffu, sum[0], d);
+      sum[1] += __shfl_xor_sync(0xffffffffu, sum[1], d);
+    }
+
+    if constexpr (C::kKeyWarps > 1) {
+      // Join the warps that share rows: scale to the common maximum, then add
+      // the accumulators, the upper half of the warps to the lower, until one is left.
+      if (tq == 0) {
+        row_stats[warp * 16 + g] = make_float2(top[0], sum[0]);
+        row_stats[warp * 16 + g + 8] = make_float2(top[1], sum[1]);
+      }
+      named_barrier(1, 128);
+      float f[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        float m = -INFINITY, l = 0.0f;
+#pragma unroll
+        for (int w = 0; w < C::kKeyWarps; ++w) m = fmaxf(m, row_stats[(w * C::kRowWarps + rw) * 16 + g + i * 8].x);
+        const float z = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+        for (int w = 0; w < C::kKeyWarps; ++w) {
+          const float2 st = row_stats[(w * C::kRowWarps + rw) * 16 + g + i * 8];
+          l = fmaf(st.y, ex2(st.x - z), l);
+        }
+        f[i] = ex2(top[i] - z);
+        top[i] = m;
+        sum[i] = l;
+      }
+#pragma unroll
+      for (int i = 0; i < D / 8; ++i) {
+        acc[i][0] *= f[0];
+        acc[i][1] *= f[0];
+        acc[i][2] *= f[1];
+        acc[i][3] *= f[1];
+      }
+#pragma unroll
+      for (int step = C::kKeyWarps / 2; step >= 1; step >>= 1) {
+        // Element i of lane l at i * 32 + l: no bank is hit twice.
+        if (kw >= step && kw < 2 * step) {
+          float* dst = join + ((kw - step) * C::kRowWarps + rw) * (16 * D);
+#pragma unroll
+          for (int i = 0; i < D / 8; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) dst[(i * 4 + j) * 32 + lane] = acc[i][j];
+        }
+        named_barrier(1, 128);
+        if (kw < step) {
+          const float* src = join + (kw * C::kRowWarps + rw) * (16 * D);
+#pragma unroll
+          for (int i = 0; i < D / 8; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[i][j] += src[(i * 4 + j) * 32 + lane];
+        }
+        named_barrier(1, 128);
+      }
+    }
+    if (kw == 0) {
+      const bool whole = s.begin == 0 && s.end == s.of;
+      const bool direct = whole && (pass.mode == kAttnConcat || (pass.mode == kAttnOwn && a.groups == 0));
+      if (direct) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          if (token[i] < 0) continue;
+          const float inv = sum[i] > 0.0f ? 1.0f / sum[i] : 0.0f;
+          uint32_t* dst = reinterpret_cast<uint32_t*>(a.out + token[i] * a.out_token + head[i] * a.out_head);
+#pragma unroll
+          for (int c = 0; c < D / 8; ++c)
+            dst[c * 4 + tq] = pack16<kBf16>(acc[c][2 * i] * inv, acc[c][2 * i + 1] * inv);
+        }
+      } else {
+        const int slot = pass.dense ? static_cast<int>(blockIdx.x) + s.item : 2 * static_cast<int>(blockIdx.x) + !first;
+        if (slot < pass.slots) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const long long r = static_cast<long long>(slot) * R + rw * 16 + g + i * 8;
+            if (tq == 0) pass.stats[r] = make_float2(top[i], sum[i]);
+            float2* dst = reinterpret_cast<float2*>(pass.acc + r * D);
+#pragma unroll
+            for (int c = 0; c < D / 8; ++c) dst[c * 4 + tq] = make_float2(acc[c][2 * i], acc[c][2 * i + 1]);
+          }
+        } else {
+          record_error(kErrBadPage);  // starts that overlap: more items than there are tokens
+        }
+      }
+    }
+    first = false;
+  }
+}
+
+// ------------------------------------------------------------ joining segments
+
+// What a pass left of one row: its segments are those of CTAs c0..c1 at the slots below.
+struct AttnRowParts {
+  int c0, c1, item, row;  // c1 < c0: nothing
+  int begins;             // the item's first pair is CTA c0's first
+};
+
+__device__ __forceinline__ int attn_owner(int total, int ctas, int w) {
+  int c = static_cast<int>(static_cast<long long>(w) * ctas / total);
+  while (c + 1 < ctas && attn_share(total, ctas, c + 1) <= w) ++c;
+  while (c > 0 && attn_share(total, ctas, c) > w) --c;
+  return c;
+}
+
+__device__ __forceinline__ AttnRowParts attn_row_parts(const AttnArgs& a, const AttnPass& pass, int e, int token, int h,
+                                                       int hr, int lane) {
+  AttnRowParts p = {0, -1, 0, 0, 0};
+  const int R = pass.rows, KT = pass.keys;
+  const AttnEntity ent = attn_entity(a, pass.mode, e);
+  const int row = (token - ent.tok0) * a.ratio + hr;
+  if (row < 0 || row >= ent.ntok * a.ratio) return p;
+  const int t = row / R, k = attn_key_tiles(ent, a.ratio, t, R, KT);
+  if (k == 0) return p;
+  const int total = pass.plan[pass.entities];
+  int before = 0;
+  if (ent.causal && ent.ntok > 1) {
+    for (int i = lane; i < t; i += 32) before += attn_key_tiles(ent, a.ratio, i, R, KT);
+    before = warp_sum_int(before);
+  } else {
+    before = t * k;
+  }
+  const int w = pass.plan[e] + before * a.kv_heads + h * k;
+  p.row = row - t * R;
+  p.item = pass.plan[pass.entities + 1 + e] + t * a.kv_heads + h;
+  const int ctas = min(pass.ctas, total);
+  p.c0 = attn_owner(total, ctas, w);
+  p.c1 = attn_owner(total, ctas, w + k - 1);
+  p.begins = attn_share(total, ctas, p.c0) == w;
+  return p;
+}
+
+// Adds a pass's segments of one row into (top, sum, acc); a lane holds D / 32 consecutive elements.
+template <int D>
+__device__ __forceinline__ void attn_add_parts(const AttnPass& pass, const AttnRowParts& p, int lane, float& top,
+                                               float& sum, float (&acc)[D / 32]) {
+  constexpr int N = D / 32;
+  for (int c = p.c0; c <= p.c1; ++c) {
+    const int slot = pass.dense ? c + p.item : 2 * c + (c == p.c0 && !p.begins);
+    if (slot >= pass.slots) return;
+    const long long r = static_cast<long long>(slot) * pass.rows + p.row;
+    const float2 st = pass.stats[r];
+    float x[N];
+    load_values<kTypeF32, N>(pass.acc, r * D + lane * N, x);
+    const float m = fmaxf(top, st.x), z = m == -INFINITY ? 0.0f : m;
+    const float f = ex2(top - z), fx = ex2(st.x - z);
+    top = m;
+    sum = fmaf(st.y, fx, sum * f);
+#pragma unroll
+    for (int i = 0; i < N; ++i) acc[i] = fmaf(x[i], fx, acc[i] * f);
+  }
+}
+
+// A warp per (token, query head).  Rows that one segment covers alone are in
+// out already; rows that see nothing become zeros.  first: the prefixes' pass
+// (or the only one), second: the own rows' pass where there are two.
+template <int D, bool kBf16>
+__global__ void __launch_bounds__(256) paged_merge_kernel(const AttnArgs a, const AttnPass first, const AttnPass second) {
+  pdl_wait_prerequisite();
+  pdl_launch_dependents();
+  constexpr int N = D / 32;
+  const int lane = threadIdx.x & 31, q_heads = a.kv_heads * a.ratio;
+  const long long w = static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  if (w >= static_cast<long long>(a.tokens) * q_heads) return;
+  const int token = static_cast<int>(w / q_heads), head = static_cast<int>(w % q_heads);
+  const int h = head / a.ratio, hr = head - h * a.ratio;
+  int seq = token;
+  if (a.q_start) {
+    if (token < a.q_start[0] || token >= a.q_start[a.seqs]) return;  // rows behind the last sequence stay
+    int lo = 0, hi = a.seqs;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (a.q_start[mid] <= token) lo = mid; else hi = mid;
+    }
+    seq = lo;
+  }
+  float top = -INFINITY, sum = 0.0f, acc[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) acc[i] = 0.0f;
+  auto add = [&](const AttnPass& pass, int e) {
+    attn_add_parts<D>(pass, attn_row_parts(a, pass, e, token, h, hr, lane), lane, top, sum, acc);
+  };
+  if (first.mode == kAttnBoth || first.mode == kAttnPrefix) {
+    const int g = attn_group_of(a, seq);
+    if (g >= 0) add(first, g);
+    if (first.mode == kAttnBoth)
+      add(first, a.groups + seq);
+    else
+      add(second, seq);
+  } else {
+    const AttnRowParts p = attn_row_parts(a, first, seq, token, h, hr, lane);
+    if (p.c1 == p.c0) return;  // written by its only segment
+    attn_add_parts<D>(first, p, lane, top, sum, acc);
+  }
+  const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+#pragma unroll
+  for (int i = 0; i < N; ++i) acc[i] *= inv;
+  store_values16<kBf16, N>(a.out + token * a.out_token + head * a.out_head + lane * N, acc);
+}
+
+}  // namespace mllb
