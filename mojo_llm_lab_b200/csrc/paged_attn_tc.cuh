@@ -1,0 +1,412 @@
+// Attention over the paged cache where a key serves many query rows (a long
+// prefix under a batch's queries, prompts): the products run on the
+// 5th-generation tensor cores.
+//
+// One persistent CTA per SM walks its share of the line (paged_attn.cuh) with
+// R = 256 rows an item, as two streams of 128 rows (a TMEM lane each) that use
+// the same key tiles of 128:
+//   warps 0-3, 4-7  softmax of stream 0, 1: a thread is a row
+//   warp 8          TMA copies of K and V tiles into a ring
+//   warp 9          issues the matrix instructions (lane 0), owns TMEM
+//   warps 10, 11    fill the warpgroup, whose registers the softmax takes
+// S = Q K^T goes to 128 TMEM columns a stream; the softmax reads it, writes
+// P over it in 16 bits, and P V adds to the stream's D columns of O, with P
+// read from TMEM and V from shared memory as it lies in the cache (MN-major).
+// While one stream's softmax runs, the tensor cores work for the other.
+//
+// The running maximum is moved, and O rescaled, only when a row's scores
+// outgrow it by 2^8: until then its weights are up to 2^8 instead of up to 1,
+// which the 16-bit types hold as well and fp32 sums too.  After the first
+// tiles O is hardly ever touched by the softmax warps.
+#pragma once
+
+#include "paged_attn.cuh"
+#include "prefill.cuh"
+
+namespace mllb {
+
+template <int D>
+struct AttnMany {
+  static constexpr int kRows = 256, kKeys = 128;
+  static constexpr int kThreads = 384;            // three warpgroups; warps 10, 11 have nothing to do
+  // Registers a thread: the launch's, then the softmax warpgroups' and the
+  // third's (setmaxnreg moves them; the sum must not exceed the launch's).
+  static constexpr int kRegs = 168, kSoftmaxRegs = 208, kOtherRegs = 88;
+  static_assert(2 * kSoftmaxRegs + kOtherRegs <= 3 * kRegs, "register split");
+  static constexpr int kQTile = 128 * D * 2;      // one stream's queries
+  static constexpr int kTile = kKeys * D * 2;     // a K or V tile: a ring slot
+  static constexpr int kSlots = D == 128 ? 5 : 8;
+  static constexpr int kRingOff = 2 * kQTile;
+  static constexpr int kBarOff = kRingOff + kSlots * kTile;
+  static constexpr int kBars = 2 * kSlots + 4 * 2 + 1;
+  static constexpr int kSmem = kBarOff + (kBars + 1) * 8;
+  static constexpr int kTmemCols = 512;           // S (P over it) 2 x 128, O 2 x D
+  static constexpr uint32_t kSCol = 0, kOCol = 256;
+  static_assert(kSmem <= 227 * 1024, "shared memory");
+  static_assert(kSlots * kTile >= (2 * (kAttnMaxEntities + 1) + 64) * 4, "the scan fits in the ring");
+};
+
+// Shared-memory descriptor, 128-byte swizzle.  K-major (Q, K): 8-row groups at
+// sbo; MN-major (V): 8-key groups at sbo, blocks of 64 elements at lbo.
+__device__ __forceinline__ uint64_t attn_desc(uint32_t saddr, uint32_t lbo, uint32_t sbo) {
+  return pf_smem_desc(saddr, lbo, sbo) | (2ull << 61);
+}
+
+// kind::f16 instruction descriptor: D fp32, A and B of the cache's type, M = 128.
+template <bool kBf16>
+__host__ __device__ constexpr uint32_t attn_idesc(int n, bool b_mn_major) {
+  return (1u << 4) | (kBf16 ? (1u << 7) | (1u << 10) : 0u) | (b_mn_major ? 1u << 16 : 0u) |
+         (static_cast<uint32_t>(n >> 3) << 17) | ((128u >> 4) << 24);
+}
+
+__device__ __forceinline__ void tc_mma_f16_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t add) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(add)
+      : "memory");
+}
+__device__ __forceinline__ void tc_mma_f16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t add) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+      ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(add)
+      : "memory");
+}
+
+// 32 TMEM columns of this thread's lane (issue only), and 16 columns back.
+__device__ __forceinline__ void tc_ld32(uint32_t taddr, float* v) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]),
+        "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]), "=f"(v[16]),
+        "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]), "=f"(v[24]),
+        "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tc_st16(uint32_t taddr, const uint32_t* v) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16};" ::"r"(taddr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+      "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+      : "memory");
+}
+__device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// a * b + c on two fp32 values at once.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(reinterpret_cast<uint64_t&>(d))
+      : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)), "l"(reinterpret_cast<uint64_t&>(c)));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("add.rn.f32x2 %0, %1, %2;"
+      : "=l"(reinterpret_cast<uint64_t&>(d))
+      : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
+  return d;
+}
+
+template <int D, bool kBf16>
+__global__ void __launch_bounds__(384, 1)
+    paged_attn_many_kernel(const AttnArgs a, const AttnPass pass, const __grid_constant__ CUtensorMap kmap,
+                           const __grid_constant__ CUtensorMap vmap) {
+  using C = AttnMany<D>;
+  constexpr int R = C::kRows, KT = C::kKeys, NS = C::kSlots;
+  extern __shared__ __align__(1024) uint8_t attn_smem[];
+  uint8_t* ring = attn_smem + C::kRingOff;
+  uint64_t* full = reinterpret_cast<uint64_t*>(attn_smem + C::kBarOff);  // [NS] a tile has landed
+  uint64_t* empty = full + NS;                                            // [NS] its products are done
+  uint64_t* q_full = empty + NS;                                          // [2] a stream's queries are in shared memory
+  uint64_t* s_full = q_full + 2;                                          // [2] its scores are in TMEM
+  uint64_t* p_full = s_full + 2;                                          // [2] its weights are, and O is at their scale
+  uint64_t* o_done = p_full + 2;                                          // [2] its products with V are done
+  uint64_t* drained = o_done + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drained + 1);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < NS; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&q_full[i], 128);
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], 128);
+      mbar_init(&o_done[i], 1);
+    }
+    mbar_init(drained, 1);
+    fence_mbar_init();
+    tma_prefetch_map(&kmap);
+    tma_prefetch_map(&vmap);
+  }
+  if (warp == 9) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(tmem_slot)),
+                 "r"(C::kTmemCols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  pdl_wait_prerequisite();
+  pdl_launch_dependents();
+  const AttnCursor start = attn_start<R, KT, C::kThreads>(a, pass, reinterpret_cast<int*>(ring));
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the scan used the ring
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kOtherRegs));
+    if (warp == 8) {
+      AttnWalk<R, KT> walk(a, pass, start);
+      AttnSegment s;
+      // ------------------------------------------------ copies: K and V tiles in turn, a box a lane
+      const int box_rows = min(1 << a.page_shift, KT), per_tile = KT / box_rows;
+      constexpr int kHalves = D / 64;
+      const int boxes = per_tile * kHalves;
+      int n = 0;
+      bool stuck = false;
+      while (!stuck && walk.next(&s)) {
+        for (int k = s.begin; k < s.end && !stuck; ++k) {
+          const AttnTile tile = attn_tile<KT>(s.ent, k);
+          const int p = lane % per_tile, half = lane / per_tile;
+          int page = 0;
+          if (lane < boxes) page = attn_page(a, tile, p * box_rows);
+          const int in_page = (tile.row0 + p * box_rows) & ((1 << a.page_shift) - 1);
+#pragma unroll
+          for (int is_v = 0; is_v < 2; ++is_v) {
+            const int st = n % NS;
+            if (n >= NS && !mbar_wait_bounded(&empty[st], (n / NS - 1) & 1)) {
+              record_error(kErrEmptyWaitTimeout);
+              stuck = true;
+              break;
+            }
+            if (lane == 0) mbar_arrive_expect_tx(&full[st], C::kTile);
+            __syncwarp();
+            if (lane < boxes)
+              tma_load_4d(ring + st * C::kTile + half * (KT * 128) + p * box_rows * 128, is_v ? &vmap : &kmap, half * 64,
+                          in_page, s.h, page, &full[st]);
+            ++n;
+          }
+        }
+      }
+      for (int i = max(n - NS, 0); i < n; ++i)
+        if (!mbar_wait_bounded(&full[i % NS], (i / NS) & 1)) record_error(kErrDrainTimeout);
+    } else if (warp == 9) {
+      // ------------------------------------------------ matrix instructions
+      if (lane == 0) {
+        AttnWalk<R, KT> walk(a, pass, start);
+        AttnSegment s;
+        constexpr uint32_t kQk = attn_idesc<kBf16>(KT, false), kPv = attn_idesc<kBf16>(D, true);
+        const uint32_t q_base = smem_addr(attn_smem), ring_base = smem_addr(ring);
+        int n = 0;                    // ring position of the next K tile to use
+        int qn[2] = {0, 0}, pn[2] = {0, 0};
+        bool ok = true;
+        auto wait = [&](uint64_t* bar, int phase) {
+          if (ok && !mbar_wait_bounded(bar, phase & 1)) {
+            record_error(kErrFullWaitTimeout);
+            ok = false;
+          }
+          return ok;
+        };
+        auto scores = [&](int stream, int pos) {
+          const uint32_t kt = ring_base + (pos % NS) * C::kTile, qt = q_base + stream * C::kQTile;
+#pragma unroll
+          for (int c = 0; c < D / 16; ++c) {
+            const uint32_t off = (c >> 2) * (128 * 128) + (c & 3) * 32;  // 64 elements a swizzled row, 32 bytes a step
+            tc_mma_f16_ss(tmem + C::kSCol + stream * 128, attn_desc(qt + off, 16, 1024), attn_desc(kt + off, 16, 1024), kQk,
+                          c > 0);
+          }
+          tc_commit(&s_full[stream]);
+        };
+        while (ok && walk.next(&s)) {
+          const int streams = s.ent.ntok * a.ratio - s.t * R > 128 ? 2 : 1, tiles = s.end - s.begin;
+          for (int i = 0; i < streams; ++i) wait(&q_full[i], qn[i]++);
+          wait(&full[n % NS], n / NS);
+          if (!ok) break;
+          tc_fence_after();
+          for (int i = 0; i < streams; ++i) scores(i, n);
+          tc_commit(&empty[n % NS]);
+          for (int k = 0; k < tiles; ++k, n += 2) {
+            const int vpos = n + 1, kpos = n + 2;
+            const bool more = k + 1 < tiles;
+            wait(&full[vpos % NS], vpos / NS);
+            if (more) wait(&full[kpos % NS], kpos / NS);
+            for (int i = 0; i < streams; ++i) {
+              if (!wait(&p_full[i], pn[i]++)) break;
+              tc_fence_after();
+              const uint32_t vt = ring_base + (vpos % NS) * C::kTile;
+#pragma unroll
+              for (int c = 0; c < KT / 16; ++c)
+                tc_mma_f16_ts(tmem + C::kOCol + i * 128, tmem + C::kSCol + i * 128 + c * 8,
+                              attn_desc(vt + c * 2048, KT * 128, 1024), kPv, k > 0 || c > 0);
+              tc_commit(&o_done[i]);
+              if (more) scores(i, kpos);  // over P, which the products before it have read: they run in order
+            }
+            if (!ok) break;
+            tc_commit(&empty[vpos % NS]);
+            if (more) tc_commit(&empty[kpos % NS]);
+          }
+        }
+        // Nothing is in flight when TMEM is given back.
+        tc_commit(drained);
+        if (!mbar_wait_bounded(drained, 0)) record_error(kErrDrainTimeout);
+      }
+      __syncwarp();
+    }
+  } else {
+    // ------------------------------------------------ softmax: this thread's row
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::kSoftmaxRegs));
+    AttnWalk<R, KT> walk(a, pass, start);
+    AttnSegment s;
+    const int stream = warp >> 2, r = threadIdx.x & 127;
+    const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+    const uint32_t s_col = lanes + C::kSCol + stream * 128, o_col = lanes + C::kOCol + stream * 128;
+    const float scale = fmaxf(fabsf(a.scale_log2), 1e-30f);  // q carries the sign; 0 x a masked -inf must not come up
+    const uint32_t flip = a.scale_log2 < 0.0f ? 0x80008000u : 0u;
+    uint8_t* q_row = attn_smem + stream * C::kQTile + r * 128;
+    int sn = 0, ring_pos = 0;
+    bool first = true, stuck = false;
+    auto wait = [&](uint64_t* bar, int phase) {
+      if (!stuck && !mbar_wait_bounded(bar, phase & 1)) {
+        record_error(kErrFullWaitTimeout);
+        stuck = true;
+      }
+    };
+    for (; !stuck && walk.next(&s); ring_pos += 2 * (s.end - s.begin), first = false) {
+      const int rows = s.ent.ntok * a.ratio - s.t * R;
+      if (stream && rows <= 128) continue;
+      const int row = stream * 128 + r;
+      const bool there = row < rows;
+      const int j = there ? (s.t * R + row) / a.ratio : 0;
+      const int token = s.ent.tok0 + j, head = s.h * a.ratio + (there ? s.t * R + row - j * a.ratio : 0);
+      const int limit = there ? attn_limit(s.ent, j) : 0;
+      {
+        const uint4* src = reinterpret_cast<const uint4*>(a.q + token * a.q_token + head * a.q_head);
+#pragma unroll
+        for (int c = 0; c < D / 8; ++c) {
+          uint4 v = there ? src[c] : make_uint4(0, 0, 0, 0);
+          v.x ^= flip, v.y ^= flip, v.z ^= flip, v.w ^= flip;
+          *reinterpret_cast<uint4*>(q_row + (c >> 3) * (128 * 128) + (((c & 7) ^ (r & 7)) << 4)) = v;
+        }
+        fence_proxy_async_smem();
+        mbar_arrive(&q_full[stream]);
+      }
+      float top = -INFINITY, sum = 0.0f;
+      for (int k = s.begin; k < s.end; ++k, ++sn) {
+        const AttnTile tile = attn_tile<KT>(s.ent, k);
+        const int held = tile.rows - tile.row0;
+        if (stream == 0 && held < KT) {
+          // V rows behind the end may hold anything, and a weight of zero does
+          // not make NaN vanish: they become zero before the products.
+          const int pos = ring_pos + 2 * (k - s.begin) + 1;
+          wait(&full[pos % NS], pos / NS);
+          uint8_t* vt = ring + (pos % NS) * C::kTile;
+          for (int i = threadIdx.x; i < (KT - held) * (D / 8); i += 128) {
+            const int key = held + i / (D / 8), c = i % (D / 8);
+            *reinterpret_cast<uint4*>(vt + (c >> 3) * (KT * 128) + key * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
+          }
+          fence_proxy_async_smem();
+        }
+        wait(&s_full[stream], sn);
+        tc_fence_after();
+        float x[KT];
+#pragma unroll
+        for (int c = 0; c < KT; c += 32) tc_ld32(s_col + c, x + c);
+        tc_wait_ld();
+        const int end = min(tile.own ? limit : tile.rows, tile.rows) - tile.row0;
+        if (__any_sync(0xffffffffu, end < KT)) {
+#pragma unroll
+          for (int c = 0; c < KT; ++c) x[c] = c < end ? x[c] : -INFINITY;
+        }
+        float m = x[0];
+#pragma unroll
+        for (int c = 1; c < KT; ++c) m = fmaxf(m, x[c]);
+        m *= scale;
+        if (__any_sync(0xffffffffu, m > top + 8.0f)) {
+          const float z = fmaxf(m, top), f = z == -INFINITY ? 0.0f : ex2(top - z);
+          top = z;
+          sum *= f;
+          if (k > s.begin) {
+            wait(&o_done[stream], sn - 1);
+            tc_fence_after();
+#pragma unroll
+            for (int c = 0; c < D; c += 32) {
+              float o[32];
+              tc_ld32(o_col + c, o);
+              tc_wait_ld();
+#pragma unroll
+              for (int i = 0; i < 32; ++i) o[i] *= f;
+              tc_st16(o_col + c, reinterpret_cast<uint32_t*>(o));
+              tc_st16(o_col + c + 16, reinterpret_cast<uint32_t*>(o) + 16);
+            }
+          }
+        }
+        const float z = top == -INFINITY ? 0.0f : top;
+        float2 part = make_float2(0.0f, 0.0f);
+        // P in the cache's type (half a step off at most; the sum keeps the unrounded weights).
+#pragma unroll
+        for (int c = 0; c < KT; c += 32) {
+          uint32_t p[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            float2 w = fma2(make_float2(x[c + 2 * i], x[c + 2 * i + 1]), make_float2(scale, scale), make_float2(-z, -z));
+            w.x = ex2(w.x);
+            w.y = ex2(w.y);
+            part = add2(part, w);
+            p[i] = pack16<kBf16>(w.x, w.y);
+          }
+          tc_st16(s_col + c / 2, p);
+        }
+        sum += part.x + part.y;
+        tc_wait_st();
+        tc_fence_before();
+        mbar_arrive(&p_full[stream]);
+      }
+      wait(&o_done[stream], sn - 1);
+      tc_fence_after();
+      const bool whole = s.begin == 0 && s.end == s.of;
+      const bool direct = whole && (pass.mode == kAttnConcat || (pass.mode == kAttnOwn && a.groups == 0));
+      const int slot = pass.dense ? static_cast<int>(blockIdx.x) + s.item : 2 * static_cast<int>(blockIdx.x) + !first;
+      const bool fits = slot < pass.slots;
+      if (!direct && !fits) record_error(kErrBadPage);
+      const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+      const long long at = static_cast<long long>(slot) * R + row;
+      if (!direct && fits) pass.stats[at] = make_float2(top, sum);
+#pragma unroll
+      for (int c = 0; c < D; c += 32) {
+        float o[32];
+        tc_ld32(o_col + c, o);
+        tc_wait_ld();
+        if (direct && there) {
+          uint4* dst = reinterpret_cast<uint4*>(a.out + token * a.out_token + head * a.out_head + c);
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            dst[i] = make_uint4(pack16<kBf16>(o[8 * i] * inv, o[8 * i + 1] * inv),
+                                pack16<kBf16>(o[8 * i + 2] * inv, o[8 * i + 3] * inv),
+                                pack16<kBf16>(o[8 * i + 4] * inv, o[8 * i + 5] * inv),
+                                pack16<kBf16>(o[8 * i + 6] * inv, o[8 * i + 7] * inv));
+        } else if (!direct && fits) {
+          float4* dst = reinterpret_cast<float4*>(pass.acc + at * D + c);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) dst[i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+        }
+      }
+      tc_fence_before();  // the next item's products write O
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 9) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::kTmemCols) : "memory");
+  }
+}
+
+}  // namespace mllb

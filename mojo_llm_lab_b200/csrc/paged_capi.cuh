@@ -6,6 +6,7 @@
 #include "beam.cuh"
 #include "paged.cuh"
 #include "paged_attn.cuh"
+#include "paged_attn_tc.cuh"
 
 namespace {
 
@@ -112,7 +113,11 @@ struct PagedPlan {
   int64_t plan_off[2], stats_off[2], acc_off[2], bytes;
 };
 
-int few_rows(int64_t rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : 64; }
+// Row tile for entities of `rows` query rows: up to 64 the kernel for few rows
+// a key, in its narrowest shape that holds them; beyond, the tensor cores'.
+int tile_rows(int64_t rows) {
+  return rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : mllb::AttnMany<128>::kRows;
+}
 
 // Mean query rows (tokens x query heads of a KV head) of a sequence and of a
 // group decide the shape.  A sequence with a row tile's worth of rows shares
@@ -128,27 +133,28 @@ int paged_plan(int64_t tokens, int64_t q_heads, int64_t kv_heads, int64_t head_d
   p->passes = 1;
   if (groups == 0 || groups >= seqs || seq_rows >= 64) {
     p->mode[0] = groups ? mllb::kAttnConcat : mllb::kAttnOwn;
-    p->rows[0] = few_rows(seq_rows);
+    p->rows[0] = tile_rows(seq_rows);
     p->entities[0] = static_cast<int>(seqs);
   } else if (group_rows <= 64) {
     p->mode[0] = mllb::kAttnBoth;
-    p->rows[0] = few_rows(group_rows);
+    p->rows[0] = tile_rows(group_rows);
     p->entities[0] = static_cast<int>(groups + seqs);
     p->dense[0] = 1;
   } else {
     p->passes = 2;
     p->mode[0] = mllb::kAttnPrefix;
-    p->rows[0] = 64;
+    p->rows[0] = tile_rows(group_rows);
     p->entities[0] = static_cast<int>(groups);
     p->mode[1] = mllb::kAttnOwn;
-    p->rows[1] = few_rows(seq_rows);
+    p->rows[1] = tile_rows(seq_rows);
     p->entities[1] = static_cast<int>(seqs);
     p->dense[0] = p->dense[1] = 1;
   }
   int64_t at = 0;
   for (int i = 0; i < p->passes; ++i) {
-    p->keys[i] = 64;
-    p->ctas[i] = 2 * sm_count(dev);
+    const bool many = p->rows[i] > 64;
+    p->keys[i] = many ? mllb::AttnMany<128>::kKeys : mllb::AttnFew<128, 16>::kKeys;
+    p->ctas[i] = many ? sm_count(dev) : 2 * sm_count(dev);
     // Items: every entity's last row tile may be part full.
     const int64_t covers = p->mode[i] == mllb::kAttnBoth && groups ? 2 : 1;
     const int64_t items = kv_heads * (covers * ((tokens * ratio + p->rows[i] - 1) / p->rows[i]) + p->entities[i]);
@@ -190,13 +196,36 @@ int launch_few(const mllb::AttnArgs& a, const mllb::AttnPass& pass, const CUtens
                   "paged attention kernel");
 }
 
+template <typename Kernel>
+int registers_of(Kernel kernel) {
+  cudaFuncAttributes attr = {};
+  return cudaFuncGetAttributes(&attr, kernel) == cudaSuccess ? attr.numRegs : 0;
+}
+
+template <int D>
+int launch_many(const mllb::AttnArgs& a, const mllb::AttnPass& pass, const CUtensorMap& k, const CUtensorMap& v, bool bf16,
+                int dev, cudaStream_t stream, bool pdl) {
+  using C = mllb::AttnMany<D>;
+  auto kernel = bf16 ? mllb::paged_attn_many_kernel<D, true> : mllb::paged_attn_many_kernel<D, false>;
+  int grid, per_sm, rc;
+  if ((rc = stream_grid(kernel, C::kSmem, C::kThreads, dev, pass.ctas, &grid, &per_sm))) return rc;
+  // The warpgroups share out the launch's registers; with fewer than that they would wait for more for good.
+  static const int regs[2] = {registers_of(mllb::paged_attn_many_kernel<D, false>),
+                              registers_of(mllb::paged_attn_many_kernel<D, true>)};
+  if (regs[bf16] < C::kRegs) return fail(MLLB_ECUDA, "paged attention kernel built with %d registers", regs[bf16]);
+  return launched(launch(kernel, dim3(static_cast<unsigned>(pass.ctas)), dim3(C::kThreads), C::kSmem, stream, pdl, a, pass,
+                         k, v),
+                  "paged attention kernel (tensor cores)");
+}
+
 template <int D>
 int launch_attn(const mllb::AttnArgs& a, const mllb::AttnPass& pass, const CUtensorMap& k, const CUtensorMap& v, bool bf16,
                 int dev, cudaStream_t stream, bool pdl) {
   switch (pass.rows) {
     case 16: return launch_few<D, 16>(a, pass, k, v, bf16, dev, stream, pdl);
     case 32: return launch_few<D, 32>(a, pass, k, v, bf16, dev, stream, pdl);
-    default: return launch_few<D, 64>(a, pass, k, v, bf16, dev, stream, pdl);
+    case 64: return launch_few<D, 64>(a, pass, k, v, bf16, dev, stream, pdl);
+    default: return launch_many<D>(a, pass, k, v, bf16, dev, stream, pdl);
   }
 }
 
