@@ -15,10 +15,12 @@
 // (each CTA adds them up for itself), so a captured graph stays right while
 // they grow.
 //
-// A CTA's share of an item is a segment.  An item with one segment and
-// nothing else to add is written to out at once; otherwise segments leave
-// (maximum, sum, unnormalised accumulator) in fp32 in the workspace, and
-// paged_merge_kernel joins a row's segments.
+// A CTA's share of an item is a segment.  Where an item's rows get nothing from
+// elsewhere, an item of one segment is written to out at once; other segments
+// leave (maximum, sum, unnormalised accumulator) in fp32 in the workspace.
+// paged_join_kernel joins the items that were cut (at most one for each CTA);
+// where prefixes and own rows run apart, paged_merge_kernel joins all of a
+// row's segments.
 #pragma once
 
 #include <cuda.h>
@@ -56,9 +58,16 @@ struct AttnPass {
   int dense;       // 1: segment of CTA c and item i at slot c + i; 0: at 2 c (a CTA's first) or 2 c + 1
   int slots;       // capacity of the workspace
   int rows, keys;  // R and KT of the kernel that ran it (for the merge)
-  int32_t* plan;   // [2][entities + 1]: key tiles and items before each entity (for the merge)
+  // dense: [2][entities + 1], key tiles and items before each entity; otherwise
+  // [ctas] AttnCut.  For the kernel that joins.
+  int32_t* plan;
   float* acc;      // [slots][R][D]
   float2* stats;   // [slots][R] (maximum in powers of two, sum)
+};
+
+// The item that CTA c began and did not end (of 0: none).
+struct AttnCut {
+  int e, t, h, end, of, slot, total, pad;
 };
 
 struct AttnEntity {
@@ -128,10 +137,12 @@ __device__ __forceinline__ int attn_row_tiles(const AttnEntity& n, int ratio, in
   return (n.ntok * ratio + R - 1) / R;
 }
 
-// Key tiles of row tile t: the prefix's, then the own rows' up to the last token's limit.
-__device__ __forceinline__ int attn_key_tiles(const AttnEntity& n, int ratio, int t, int R, int KT) {
+// Key tiles of row tile t: the prefix's, then the own rows' up to the last
+// token's limit.  least 1 makes an item of rows that see nothing, too (one
+// masked tile), so that their zeros are written like other rows.
+__device__ __forceinline__ int attn_key_tiles(const AttnEntity& n, int ratio, int t, int R, int KT, int least) {
   const int last = min(n.ntok * ratio, (t + 1) * R) - 1;
-  return (n.plen + KT - 1) / KT + (attn_limit(n, last / ratio) + KT - 1) / KT;
+  return max((n.plen + KT - 1) / KT + (attn_limit(n, last / ratio) + KT - 1) / KT, least);
 }
 
 // First pair of CTA c's share.  No more CTAs take part than there are pairs,
@@ -142,6 +153,7 @@ __device__ __forceinline__ int attn_share(int total, int ctas, int c) {
 
 // Where a CTA's share starts, and how far it goes.
 struct AttnCursor {
+  int total;       // all pairs
   int left;        // key tiles left in the share
   int e, t, h;     // entity, row tile, KV head
   int begin;       // first key tile of the segment
@@ -149,8 +161,8 @@ struct AttnCursor {
 };
 
 // Adds up all entities' work and finds this CTA's share.  All threads of the
-// CTA call it; `scan` is shared scratch of 2 (entities + 1) + 64 ints.  CTA 0
-// also leaves the sums in pass.plan.
+// CTA call it; `scan` is shared scratch of 2 (entities + 1) + 64 ints.  For a
+// dense pass CTA 0 leaves the sums in pass.plan.
 template <int R, int KT, int kThreads>
 __device__ __forceinline__ AttnCursor attn_start(const AttnArgs& a, const AttnPass& pass, int* scan) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -166,9 +178,9 @@ __device__ __forceinline__ AttnCursor attn_start(const AttnArgs& a, const AttnPa
       const int t = attn_row_tiles(ent, a.ratio, R);
       if (t > 0) {
         if (ent.causal && ent.ntok > 1)
-          for (int i = 0; i < t; ++i) w += attn_key_tiles(ent, a.ratio, i, R, KT);
+          for (int i = 0; i < t; ++i) w += attn_key_tiles(ent, a.ratio, i, R, KT, !pass.dense);
         else
-          w = t * attn_key_tiles(ent, a.ratio, 0, R, KT);
+          w = t * attn_key_tiles(ent, a.ratio, 0, R, KT, !pass.dense);
       }
       w *= a.kv_heads;
       n = t * a.kv_heads;
@@ -198,9 +210,10 @@ __device__ __forceinline__ AttnCursor attn_start(const AttnArgs& a, const AttnPa
     items[pass.entities] = items_before;
   }
   __syncthreads();
-  if (blockIdx.x == 0)
+  if (blockIdx.x == 0 && pass.dense)
     for (int i = tid; i < 2 * (pass.entities + 1); i += kThreads) pass.plan[i] = scan[i];
   AttnCursor c;
+  c.total = tiles_before;
   const int ctas = min(pass.ctas, tiles_before);
   const int w0 = attn_share(tiles_before, max(ctas, 1), blockIdx.x);
   c.left = static_cast<int>(blockIdx.x) < ctas ? attn_share(tiles_before, ctas, blockIdx.x + 1) - w0 : 0;
@@ -213,11 +226,11 @@ __device__ __forceinline__ AttnCursor attn_start(const AttnArgs& a, const AttnPa
     }
     c.e = lo;
     const AttnEntity ent = attn_entity(a, pass.mode, lo);
-    int rest = w0 - tiles[lo], k = attn_key_tiles(ent, a.ratio, 0, R, KT);
+    int rest = w0 - tiles[lo], k = attn_key_tiles(ent, a.ratio, 0, R, KT, !pass.dense);
     if (ent.causal && ent.ntok > 1) {
       while (rest >= a.kv_heads * k) {
         rest -= a.kv_heads * k;
-        k = attn_key_tiles(ent, a.ratio, ++c.t, R, KT);
+        k = attn_key_tiles(ent, a.ratio, ++c.t, R, KT, !pass.dense);
       }
     } else {
       c.t = rest / (a.kv_heads * k);
@@ -235,17 +248,17 @@ __device__ __forceinline__ AttnCursor attn_start(const AttnArgs& a, const AttnPa
 struct AttnSegment {
   AttnEntity ent;
   int t, h, begin, end;  // row tile, KV head, key tiles [begin, end) of `of`
-  int of, item;
+  int of, item, entity;
 };
 
 template <int R, int KT>
 struct AttnWalk {
   const AttnArgs& a;
-  int mode, entities;
+  int mode, entities, least;
   AttnCursor c;
   AttnEntity ent;
   __device__ AttnWalk(const AttnArgs& args, const AttnPass& pass, const AttnCursor& start)
-      : a(args), mode(pass.mode), entities(pass.entities), c(start) {
+      : a(args), mode(pass.mode), entities(pass.entities), least(!pass.dense), c(start) {
     if (c.left > 0) ent = attn_entity(a, mode, c.e);
   }
   __device__ bool next(AttnSegment* s) {
@@ -254,7 +267,7 @@ struct AttnWalk {
     for (;;) {  // skip row tiles that see nothing and entities without rows
       const int tiles = attn_row_tiles(ent, a.ratio, R);
       if (c.t < tiles) {
-        k = attn_key_tiles(ent, a.ratio, c.t, R, KT);
+        k = attn_key_tiles(ent, a.ratio, c.t, R, KT, least);
         if (k > 0) break;
         ++c.t;
         c.item += a.kv_heads;
@@ -271,6 +284,7 @@ struct AttnWalk {
     s->end = min(k, c.begin + c.left);
     s->of = k;
     s->item = c.item;
+    s->entity = c.e;
     c.left -= s->end - s->begin;
     c.begin = 0;
     ++c.item;
@@ -278,6 +292,14 @@ struct AttnWalk {
     return true;
   }
 };
+
+// What a CTA leaves for paged_join_kernel, from its last segment (any: it had one).
+__device__ __forceinline__ void attn_leave_cut(const AttnPass& pass, const AttnCursor& start, const AttnSegment& s, bool any,
+                                               int segments) {
+  const bool cut = any && s.begin == 0 && s.end < s.of;
+  reinterpret_cast<AttnCut*>(pass.plan)[blockIdx.x] = {
+      s.entity, s.t, s.h, s.end, cut ? s.of : 0, 2 * static_cast<int>(blockIdx.x) + (segments > 1), start.total, 0};
+}
 
 // Key tile k of an entity: which table, its first row there, and how many rows that table's part has.
 struct AttnTile {
@@ -410,9 +432,11 @@ __global__ void __launch_bounds__(160, 2)
     const int box_rows = min(1 << a.page_shift, KT), per_tile = KT / box_rows;
     constexpr int kHalves = D / 64;
     const int boxes = per_tile * kHalves * 2;
-    int n = 0;
+    int n = 0, segments = 0;
     bool stuck = false;
+    s = {};
     while (!stuck && walk.next(&s)) {
+      ++segments;
       for (int k = s.begin; k < s.end; ++k, ++n) {
         const AttnTile tile = attn_tile<KT>(s.ent, k);
         const int p = lane % per_tile, rest = lane / per_tile, half = rest % kHalves, is_v = rest / kHalves;
@@ -432,6 +456,7 @@ __global__ void __launch_bounds__(160, 2)
                       is_v ? &vmap : &kmap, half * 64, in_page, s.h, page, &full[st]);
       }
     }
+    if (!pass.dense && lane == 0) attn_leave_cut(pass, start, s, segments > 0, segments);
     // The last copies land before the CTA's shared memory is given back.
     for (int i = max(n - C::kStages, 0); i < n; ++i)
       if (!mbar_wait_bounded(&full[i % C::kStages], (i / C::kStages) & 1)) record_error(kErrDrainTimeout);
@@ -618,7 +643,7 @@ __global__ void __launch_bounds__(160, 2)
     }
     if (kw == 0) {
       const bool whole = s.begin == 0 && s.end == s.of;
-      const bool direct = whole && (pass.mode == kAttnConcat || (pass.mode == kAttnOwn && a.groups == 0));
+      const bool direct = whole && !pass.dense;
       if (direct) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
@@ -654,7 +679,6 @@ __global__ void __launch_bounds__(160, 2)
 // What a pass left of one row: its segments are those of CTAs c0..c1 at the slots below.
 struct AttnRowParts {
   int c0, c1, item, row;  // c1 < c0: nothing
-  int begins;             // the item's first pair is CTA c0's first
 };
 
 __device__ __forceinline__ int attn_owner(int total, int ctas, int w) {
@@ -666,17 +690,17 @@ __device__ __forceinline__ int attn_owner(int total, int ctas, int w) {
 
 __device__ __forceinline__ AttnRowParts attn_row_parts(const AttnArgs& a, const AttnPass& pass, int e, int token, int h,
                                                        int hr, int lane) {
-  AttnRowParts p = {0, -1, 0, 0, 0};
+  AttnRowParts p = {0, -1, 0, 0};
   const int R = pass.rows, KT = pass.keys;
   const AttnEntity ent = attn_entity(a, pass.mode, e);
   const int row = (token - ent.tok0) * a.ratio + hr;
   if (row < 0 || row >= ent.ntok * a.ratio) return p;
-  const int t = row / R, k = attn_key_tiles(ent, a.ratio, t, R, KT);
+  const int t = row / R, k = attn_key_tiles(ent, a.ratio, t, R, KT, !pass.dense);
   if (k == 0) return p;
   const int total = pass.plan[pass.entities];
   int before = 0;
   if (ent.causal && ent.ntok > 1) {
-    for (int i = lane; i < t; i += 32) before += attn_key_tiles(ent, a.ratio, i, R, KT);
+    for (int i = lane; i < t; i += 32) before += attn_key_tiles(ent, a.ratio, i, R, KT, !pass.dense);
     before = warp_sum_int(before);
   } else {
     before = t * k;
@@ -687,39 +711,79 @@ __device__ __forceinline__ AttnRowParts attn_row_parts(const AttnArgs& a, const 
   const int ctas = min(pass.ctas, total);
   p.c0 = attn_owner(total, ctas, w);
   p.c1 = attn_owner(total, ctas, w + k - 1);
-  p.begins = attn_share(total, ctas, p.c0) == w;
   return p;
 }
 
-// Adds a pass's segments of one row into (top, sum, acc); a lane holds D / 32 consecutive elements.
+// Adds one segment of a row into (top, sum, acc); a lane holds D / 32 consecutive elements.
+template <int D>
+__device__ __forceinline__ void attn_add_segment(const AttnPass& pass, int slot, int row, int lane, float& top, float& sum,
+                                                 float (&acc)[D / 32]) {
+  constexpr int N = D / 32;
+  if (slot >= pass.slots) return;
+  const long long r = static_cast<long long>(slot) * pass.rows + row;
+  const float2 st = pass.stats[r];
+  float x[N];
+  load_values<kTypeF32, N>(pass.acc, r * D + lane * N, x);
+  const float m = fmaxf(top, st.x), z = m == -INFINITY ? 0.0f : m;
+  const float f = ex2(top - z), fx = ex2(st.x - z);
+  top = m;
+  sum = fmaf(st.y, fx, sum * f);
+#pragma unroll
+  for (int i = 0; i < N; ++i) acc[i] = fmaf(x[i], fx, acc[i] * f);
+}
+
+// The result of a row's segments; zeros where there was nothing to see.
+template <int D, bool kBf16>
+__device__ __forceinline__ void attn_store_row(const AttnArgs& a, int token, int head, int lane, float sum,
+                                               float (&acc)[D / 32]) {
+  constexpr int N = D / 32;
+  const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+#pragma unroll
+  for (int i = 0; i < N; ++i) acc[i] *= inv;
+  store_values16<kBf16, N>(a.out + token * a.out_token + head * a.out_head + lane * N, acc);
+}
+
+// Adds a pass's segments of one row.
 template <int D>
 __device__ __forceinline__ void attn_add_parts(const AttnPass& pass, const AttnRowParts& p, int lane, float& top,
                                                float& sum, float (&acc)[D / 32]) {
-  constexpr int N = D / 32;
   for (int c = p.c0; c <= p.c1; ++c) {
-    const int slot = pass.dense ? c + p.item : 2 * c + (c == p.c0 && !p.begins);
-    if (slot >= pass.slots) return;
-    const long long r = static_cast<long long>(slot) * pass.rows + p.row;
-    const float2 st = pass.stats[r];
-    float x[N];
-    load_values<kTypeF32, N>(pass.acc, r * D + lane * N, x);
-    const float m = fmaxf(top, st.x), z = m == -INFINITY ? 0.0f : m;
-    const float f = ex2(top - z), fx = ex2(st.x - z);
-    top = m;
-    sum = fmaf(st.y, fx, sum * f);
-#pragma unroll
-    for (int i = 0; i < N; ++i) acc[i] = fmaf(x[i], fx, acc[i] * f);
+    attn_add_segment<D>(pass, c + p.item, p.row, lane, top, sum, acc);
   }
 }
 
-// A warp per (token, query head).  Rows that one segment covers alone are in
-// out already; rows that see nothing become zeros.  first: the prefixes' pass
-// (or the only one), second: the own rows' pass where there are two.
+// Joins the item that CTA c began and others went on with: their segments of
+// it are the first ones of their shares.  Grid (CTA c, 8 rows), a warp a row.
+template <int D, bool kBf16>
+__global__ void __launch_bounds__(256) paged_join_kernel(const AttnArgs a, const AttnPass pass) {
+  pdl_wait_prerequisite();
+  pdl_launch_dependents();
+  const AttnCut cut = reinterpret_cast<const AttnCut*>(pass.plan)[blockIdx.x];
+  if (cut.of == 0) return;
+  const AttnEntity ent = attn_entity(a, pass.mode, cut.e);
+  const int lane = threadIdx.x & 31, row = blockIdx.y * 8 + (threadIdx.x >> 5), at = cut.t * pass.rows + row;
+  if (at >= ent.ntok * a.ratio) return;
+  float top = -INFINITY, sum = 0.0f, acc[D / 32];
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i) acc[i] = 0.0f;
+  attn_add_segment<D>(pass, cut.slot, row, lane, top, sum, acc);
+  const int ctas = min(pass.ctas, cut.total);
+  int left = cut.of - cut.end;
+  for (int c = blockIdx.x + 1; left > 0 && c < ctas; ++c) {
+    attn_add_segment<D>(pass, 2 * c, row, lane, top, sum, acc);
+    left -= attn_share(cut.total, ctas, c + 1) - attn_share(cut.total, ctas, c);
+  }
+  const int j = at / a.ratio;
+  attn_store_row<D, kBf16>(a, ent.tok0 + j, cut.h * a.ratio + at - j * a.ratio, lane, sum, acc);
+}
+
+// Prefixes apart from own rows: a warp per (token, query head) joins all
+// segments of both.  Rows that see nothing become zeros.  first: the prefixes'
+// pass, or the one of both; second: the own rows' pass where there are two.
 template <int D, bool kBf16>
 __global__ void __launch_bounds__(256) paged_merge_kernel(const AttnArgs a, const AttnPass first, const AttnPass second) {
   pdl_wait_prerequisite();
   pdl_launch_dependents();
-  constexpr int N = D / 32;
   const int lane = threadIdx.x & 31, q_heads = a.kv_heads * a.ratio;
   const long long w = static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5);
   if (w >= static_cast<long long>(a.tokens) * q_heads) return;
@@ -735,28 +799,19 @@ __global__ void __launch_bounds__(256) paged_merge_kernel(const AttnArgs a, cons
     }
     seq = lo;
   }
-  float top = -INFINITY, sum = 0.0f, acc[N];
+  float top = -INFINITY, sum = 0.0f, acc[D / 32];
 #pragma unroll
-  for (int i = 0; i < N; ++i) acc[i] = 0.0f;
+  for (int i = 0; i < D / 32; ++i) acc[i] = 0.0f;
   auto add = [&](const AttnPass& pass, int e) {
     attn_add_parts<D>(pass, attn_row_parts(a, pass, e, token, h, hr, lane), lane, top, sum, acc);
   };
-  if (first.mode == kAttnBoth || first.mode == kAttnPrefix) {
-    const int g = attn_group_of(a, seq);
-    if (g >= 0) add(first, g);
-    if (first.mode == kAttnBoth)
-      add(first, a.groups + seq);
-    else
-      add(second, seq);
-  } else {
-    const AttnRowParts p = attn_row_parts(a, first, seq, token, h, hr, lane);
-    if (p.c1 == p.c0) return;  // written by its only segment
-    attn_add_parts<D>(first, p, lane, top, sum, acc);
-  }
-  const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
-#pragma unroll
-  for (int i = 0; i < N; ++i) acc[i] *= inv;
-  store_values16<kBf16, N>(a.out + token * a.out_token + head * a.out_head + lane * N, acc);
+  const int g = attn_group_of(a, seq);
+  if (g >= 0) add(first, g);
+  if (first.mode == kAttnBoth)
+    add(first, a.groups + seq);
+  else
+    add(second, seq);
+  attn_store_row<D, kBf16>(a, token, head, lane, sum, acc);
 }
 
 }  // namespace mllb

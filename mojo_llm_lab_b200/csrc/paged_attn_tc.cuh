@@ -170,9 +170,11 @@ __global__ void __launch_bounds__(384, 1)
       const int box_rows = min(1 << a.page_shift, KT), per_tile = KT / box_rows;
       constexpr int kHalves = D / 64;
       const int boxes = per_tile * kHalves;
-      int n = 0;
+      int n = 0, segments = 0;
       bool stuck = false;
+      s = {};
       while (!stuck && walk.next(&s)) {
+        ++segments;
         for (int k = s.begin; k < s.end && !stuck; ++k) {
           const AttnTile tile = attn_tile<KT>(s.ent, k);
           const int p = lane % per_tile, half = lane / per_tile;
@@ -196,6 +198,7 @@ __global__ void __launch_bounds__(384, 1)
           }
         }
       }
+      if (!pass.dense && lane == 0) attn_leave_cut(pass, start, s, segments > 0, segments);
       for (int i = max(n - NS, 0); i < n; ++i)
         if (!mbar_wait_bounded(&full[i % NS], (i / NS) & 1)) record_error(kErrDrainTimeout);
     } else if (warp == 9) {
@@ -325,10 +328,15 @@ __global__ void __launch_bounds__(384, 1)
 #pragma unroll
           for (int c = 0; c < KT; ++c) x[c] = c < end ? x[c] : -INFINITY;
         }
-        float m = x[0];
+        // Four chains of three-input maxima.
+        float mc[4] = {x[0], x[1], x[2], x[3]};
 #pragma unroll
-        for (int c = 1; c < KT; ++c) m = fmaxf(m, x[c]);
-        m *= scale;
+        for (int c = 4; c + 8 <= KT; c += 8)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) mc[i] = fmaxf(fmaxf(mc[i], x[c + i]), x[c + 4 + i]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) mc[i] = fmaxf(mc[i], x[KT - 4 + i]);
+        const float m = fmaxf(fmaxf(mc[0], mc[1]), fmaxf(mc[2], mc[3])) * scale;
         if (__any_sync(0xffffffffu, m > top + 8.0f)) {
           const float z = fmaxf(m, top), f = z == -INFINITY ? 0.0f : ex2(top - z);
           top = z;
@@ -349,7 +357,7 @@ __global__ void __launch_bounds__(384, 1)
           }
         }
         const float z = top == -INFINITY ? 0.0f : top;
-        float2 part = make_float2(0.0f, 0.0f);
+        float2 part[4] = {};
         // P in the cache's type (half a step off at most; the sum keeps the unrounded weights).
 #pragma unroll
         for (int c = 0; c < KT; c += 32) {
@@ -359,12 +367,13 @@ __global__ void __launch_bounds__(384, 1)
             float2 w = fma2(make_float2(x[c + 2 * i], x[c + 2 * i + 1]), make_float2(scale, scale), make_float2(-z, -z));
             w.x = ex2(w.x);
             w.y = ex2(w.y);
-            part = add2(part, w);
+            part[i & 3] = add2(part[i & 3], w);
             p[i] = pack16<kBf16>(w.x, w.y);
           }
           tc_st16(s_col + c / 2, p);
         }
-        sum += part.x + part.y;
+        part[0] = add2(add2(part[0], part[1]), add2(part[2], part[3]));
+        sum += part[0].x + part[0].y;
         tc_wait_st();
         tc_fence_before();
         mbar_arrive(&p_full[stream]);
@@ -372,7 +381,7 @@ __global__ void __launch_bounds__(384, 1)
       wait(&o_done[stream], sn - 1);
       tc_fence_after();
       const bool whole = s.begin == 0 && s.end == s.of;
-      const bool direct = whole && (pass.mode == kAttnConcat || (pass.mode == kAttnOwn && a.groups == 0));
+      const bool direct = whole && !pass.dense;
       const int slot = pass.dense ? static_cast<int>(blockIdx.x) + s.item : 2 * static_cast<int>(blockIdx.x) + !first;
       const bool fits = slot < pass.slots;
       if (!direct && !fits) record_error(kErrBadPage);

@@ -162,7 +162,8 @@ int paged_plan(int64_t tokens, int64_t q_heads, int64_t kv_heads, int64_t head_d
     if (slots > (1 << 30)) return fail(MLLB_EINVAL, "too many tokens x heads");
     p->slots[i] = static_cast<int>(slots);
     p->plan_off[i] = at;
-    at += (2ll * (p->entities[i] + 1) * 4 + 255) / 256 * 256;
+    const int64_t plan = p->dense[i] ? 2ll * (p->entities[i] + 1) * 4 : p->ctas[i] * static_cast<int64_t>(sizeof(mllb::AttnCut));
+    at += (plan + 255) / 256 * 256;
     p->stats_off[i] = at;
     at += slots * p->rows[i] * 8;
     p->acc_off[i] = at;
@@ -227,6 +228,13 @@ int launch_attn(const mllb::AttnArgs& a, const mllb::AttnPass& pass, const CUten
     case 64: return launch_few<D, 64>(a, pass, k, v, bf16, dev, stream, pdl);
     default: return launch_many<D>(a, pass, k, v, bf16, dev, stream, pdl);
   }
+}
+
+template <int D>
+cudaError_t launch_join(const mllb::AttnArgs& a, const mllb::AttnPass& pass, bool bf16, cudaStream_t stream) {
+  auto kernel = bf16 ? mllb::paged_join_kernel<D, true> : mllb::paged_join_kernel<D, false>;
+  return launch(kernel, dim3(static_cast<unsigned>(pass.ctas), static_cast<unsigned>(pass.rows / 8)), dim3(256), 0, stream,
+                true, a, pass);
 }
 
 template <int D>
@@ -398,6 +406,9 @@ int mllb_paged_attention(const mllb_paged_attn* p, const mllb_paged_cache* cache
                                 : launch_attn<64>(a, pass[i], kmap, vmap, bf16, dev, s, pdl);
     if (rc) return rc;
   }
+  if (!pass[0].dense)
+    return launched(cache->head_dim == 128 ? launch_join<128>(a, pass[0], bf16, s) : launch_join<64>(a, pass[0], bf16, s),
+                    "paged join kernel");
   return launched(cache->head_dim == 128 ? launch_merge<128>(a, pass[0], pass[1], bf16, s)
                                          : launch_merge<64>(a, pass[0], pass[1], bf16, s),
                   "paged merge kernel");
