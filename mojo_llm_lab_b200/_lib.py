@@ -7,6 +7,7 @@ that fails the import error propagates.
 from __future__ import annotations
 
 import ctypes as C
+import importlib.util
 import re
 import threading
 from pathlib import Path
@@ -145,6 +146,7 @@ SIGNATURES = {
 
 _lock = threading.Lock()
 _handle = None
+_native = None
 
 
 class MllbError(RuntimeError):
@@ -174,6 +176,24 @@ def lib() -> C.CDLL:
                 raise RuntimeError("libmllb200.so ABI version mismatch")
             _handle = handle
     return _handle
+
+
+def native():
+    """The extension module lib/mllb200_torch.so (csrc/torch_ops.cpp)."""
+    global _native
+    if _native is None:
+        import torch  # noqa: F401  (its libraries are what the extension links to)
+        lib()
+        with _lock:
+            if _native is None:
+                if not _build.TORCH_EXT.exists():
+                    _build.build()
+                spec = importlib.util.spec_from_file_location("mllb200_torch", _build.TORCH_EXT)
+                module = importlib.util.module_from_spec(spec)
+                spec.loader.exec_module(module)
+                module.set_error(MllbError)
+                _native = module
+    return _native
 
 
 def check(rc: int, what: str) -> None:

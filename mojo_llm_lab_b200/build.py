@@ -11,7 +11,11 @@
                               graphs of serialised reps, ABBA arms, NVML
                               clocks, red zones; csrc/harness.cpp)
 
-Both target `-gencode arch=compute_100a,code=sm_100a` only (B200).  The build
+* lib/mllb200_torch.so      -- Python extension: tensor checks and calls of the
+                              paged-cache operators (csrc/torch_ops.cpp, host
+                              code only)
+
+The CUDA ones target `-gencode arch=compute_100a,code=sm_100a` only (B200).  The build
 is incremental on source mtimes; `python -m mojo_llm_lab_b200.build` forces it.
 """
 from __future__ import annotations
@@ -20,6 +24,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -31,6 +36,7 @@ LIB = LIBDIR / "libmllb200.so"
 CUBIN = LIBDIR / "mllb200_compat.cubin"
 INTERPOSE = LIBDIR / "libmllb200_interpose.so"
 HARNESS = LIBDIR / "mllb200_harness"
+TORCH_EXT = LIBDIR / "mllb200_torch.so"
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 COMMON = ["-O3", "-std=c++17", "-lineinfo", "-Xptxas", "-v", f"-I{INCLUDE}", f"-I{CSRC}"]
@@ -85,6 +91,20 @@ def build(force: bool = False, verbose: bool = False) -> dict:
               "-Wl,-rpath,$ORIGIN"], LIBDIR / "build_interpose.log", verbose)
         tmp.replace(INTERPOSE)
         built["interpose"] = str(INTERPOSE)
+    if force or _stale(TORCH_EXT) or TORCH_EXT.stat().st_mtime < LIB.stat().st_mtime:
+        import torch
+        torch_dir = Path(torch.__file__).resolve().parent
+        tmp = TORCH_EXT.with_suffix(".so.tmp")
+        cuda_inc = Path(nvcc()).resolve().parent.parent / "include"
+        system = [torch_dir / "include", torch_dir / "include" / "torch" / "csrc" / "api" / "include", cuda_inc,
+                  sysconfig.get_paths()["include"]]
+        _run([shutil.which("g++") or "g++", "-O2", "-std=c++20", "-fPIC", "-shared", "-Wall", f"-I{INCLUDE}",
+              *(arg for p in system for arg in ("-isystem", str(p))),
+              f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-o", str(tmp),
+              str(CSRC / "torch_ops.cpp"), f"-L{LIBDIR}", "-lmllb200", f"-L{torch_dir / 'lib'}", "-ltorch_python",
+              "-ltorch_cpu", "-lc10", "-lc10_cuda", "-Wl,-rpath,$ORIGIN"], LIBDIR / "build_torch.log", verbose)
+        tmp.replace(TORCH_EXT)
+        built["torch"] = str(TORCH_EXT)
     if force or _stale(HARNESS) or HARNESS.stat().st_mtime < LIB.stat().st_mtime:
         tmp = HARNESS.with_suffix(".tmp")
         _run([nvcc(), "-O2", "-std=c++17", f"-I{INCLUDE}", "-o", str(tmp), str(CSRC / "harness.cpp"),

@@ -44,6 +44,13 @@ __device__ __forceinline__ float2 unpack16(uint32_t w) {
   }
 }
 
+// 2^x by the special-function unit (2 units in the last place).
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 // Element types of activations and logits (MLLB_TYPE_* of the public header).
 enum : int { kTypeF32 = 0, kTypeF16 = 1, kTypeBf16 = 2 };
 

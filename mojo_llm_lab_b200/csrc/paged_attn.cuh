@@ -58,16 +58,18 @@ struct AttnPass {
   int dense;       // 1: segment of CTA c and item i at slot c + i; 0: at 2 c (a CTA's first) or 2 c + 1
   int slots;       // capacity of the workspace
   int rows, keys;  // R and KT of the kernel that ran it (for the merge)
-  // dense: [2][entities + 1], key tiles and items before each entity; otherwise
-  // [ctas] AttnCut.  For the kernel that joins.
+  // For the kernel that joins.  dense: [entities] items before each entity,
+  // then int2 [items] first and last CTA of an item; otherwise [ctas] AttnCut.
   int32_t* plan;
   float* acc;      // [slots][R][D]
   float2* stats;   // [slots][R] (maximum in powers of two, sum)
 };
 
-// The item that CTA c began and did not end (of 0: none).
+// The item that CTA c began and others went on with (segments 0: none): how
+// many segments, the slot of CTA c's, the item's first row of its entity's
+// `rows`, its KV head and the entity's first token.
 struct AttnCut {
-  int e, t, h, end, of, slot, total, pad;
+  int segments, slot, row0, rows, h, tok0, pad0, pad1;
 };
 
 struct AttnEntity {
@@ -160,31 +162,82 @@ struct AttnCursor {
   int item;        // number of the item on the line
 };
 
+// Entity e's (row tile, KV head, key tile) pairs and its items; 0 past the last.
+template <int R, int KT>
+__device__ __forceinline__ void attn_work(const AttnArgs& a, const AttnPass& pass, int e, int* pairs, int* items) {
+  int w = 0, t = 0;
+  if (e < pass.entities) {
+    const AttnEntity ent = attn_entity(a, pass.mode, e);
+    t = attn_row_tiles(ent, a.ratio, R);
+    if (ent.causal && ent.ntok > 1) {
+      for (int i = 0; i < t; ++i) w += attn_key_tiles(ent, a.ratio, i, R, KT, !pass.dense);
+    } else if (t > 0) {
+      w = t * attn_key_tiles(ent, a.ratio, 0, R, KT, !pass.dense);
+    }
+  }
+  *pairs = w * a.kv_heads;
+  *items = t * a.kv_heads;
+}
+
+// This CTA's share, which starts `rest` pairs into entity e (whose first item is `item0`).
+template <int R, int KT>
+__device__ __forceinline__ AttnCursor attn_locate(const AttnArgs& a, const AttnPass& pass, int total, int e, int rest,
+                                                  int item0) {
+  AttnCursor c = {};
+  c.total = total;
+  const int ctas = min(pass.ctas, total), cta = blockIdx.x;
+  if (cta >= ctas) return c;
+  c.left = attn_share(total, ctas, cta + 1) - attn_share(total, ctas, cta);
+  c.e = e;
+  const AttnEntity ent = attn_entity(a, pass.mode, e);
+  int k = attn_key_tiles(ent, a.ratio, 0, R, KT, !pass.dense);
+  if (ent.causal && ent.ntok > 1) {
+    while (rest >= a.kv_heads * k) {
+      rest -= a.kv_heads * k;
+      k = attn_key_tiles(ent, a.ratio, ++c.t, R, KT, !pass.dense);
+    }
+  } else {
+    c.t = rest / (a.kv_heads * k);
+    rest -= c.t * a.kv_heads * k;
+  }
+  c.h = rest / k;
+  c.begin = rest - c.h * k;
+  c.item = item0 + c.t * a.kv_heads + c.h;
+  return c;
+}
+
 // Adds up all entities' work and finds this CTA's share.  All threads of the
 // CTA call it; `scan` is shared scratch of 2 (entities + 1) + 64 ints.  For a
-// dense pass CTA 0 leaves the sums in pass.plan.
+// dense pass CTA 0 leaves the numbers of items in pass.plan.
 template <int R, int KT, int kThreads>
 __device__ __forceinline__ AttnCursor attn_start(const AttnArgs& a, const AttnPass& pass, int* scan) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   constexpr int kWarps = kThreads / 32;
+  if (pass.entities <= 32) {
+    // Few entities: every warp adds them up for itself, a lane each.
+    int w, n;
+    attn_work<R, KT>(a, pass, lane, &w, &n);
+    int ws = w, ns = n;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int wu = __shfl_up_sync(0xffffffffu, ws, d), nu = __shfl_up_sync(0xffffffffu, ns, d);
+      if (lane >= d) ws += wu, ns += nu;
+    }
+    if (blockIdx.x == 0 && pass.dense && warp == 0 && lane < pass.entities) pass.plan[lane] = ns - n;
+    const int total = __shfl_sync(0xffffffffu, ws, 31), ctas = min(pass.ctas, total);
+    const int w0 = attn_share(total, max(ctas, 1), blockIdx.x);
+    // The entity that holds pair w0: the first whose sum passes it.
+    const unsigned past = __ballot_sync(0xffffffffu, ws > w0);
+    const int e = past ? __ffs(past) - 1 : 0;
+    return attn_locate<R, KT>(a, pass, total, e, w0 - __shfl_sync(0xffffffffu, ws - w, e), __shfl_sync(0xffffffffu, ns - n, e));
+  }
   int* tiles = scan;
   int* items = scan + pass.entities + 1;
   int* part = items + pass.entities + 1;  // [2][kWarps]
   int tiles_before = 0, items_before = 0;
   for (int e0 = 0; e0 < pass.entities; e0 += kThreads) {
-    int w = 0, n = 0;
-    if (e0 + tid < pass.entities) {
-      const AttnEntity ent = attn_entity(a, pass.mode, e0 + tid);
-      const int t = attn_row_tiles(ent, a.ratio, R);
-      if (t > 0) {
-        if (ent.causal && ent.ntok > 1)
-          for (int i = 0; i < t; ++i) w += attn_key_tiles(ent, a.ratio, i, R, KT, !pass.dense);
-        else
-          w = t * attn_key_tiles(ent, a.ratio, 0, R, KT, !pass.dense);
-      }
-      w *= a.kv_heads;
-      n = t * a.kv_heads;
-    }
+    int w, n;
+    attn_work<R, KT>(a, pass, e0 + tid, &w, &n);
     int ws = w, ns = n;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
@@ -211,35 +264,14 @@ __device__ __forceinline__ AttnCursor attn_start(const AttnArgs& a, const AttnPa
   }
   __syncthreads();
   if (blockIdx.x == 0 && pass.dense)
-    for (int i = tid; i < 2 * (pass.entities + 1); i += kThreads) pass.plan[i] = scan[i];
-  AttnCursor c;
-  c.total = tiles_before;
-  const int ctas = min(pass.ctas, tiles_before);
-  const int w0 = attn_share(tiles_before, max(ctas, 1), blockIdx.x);
-  c.left = static_cast<int>(blockIdx.x) < ctas ? attn_share(tiles_before, ctas, blockIdx.x + 1) - w0 : 0;
-  c.e = c.t = c.h = c.begin = c.item = 0;
-  if (c.left > 0) {
-    int lo = 0, hi = pass.entities;  // tiles[lo] <= w0 < tiles[hi]
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (tiles[mid] <= w0) lo = mid; else hi = mid;
-    }
-    c.e = lo;
-    const AttnEntity ent = attn_entity(a, pass.mode, lo);
-    int rest = w0 - tiles[lo], k = attn_key_tiles(ent, a.ratio, 0, R, KT, !pass.dense);
-    if (ent.causal && ent.ntok > 1) {
-      while (rest >= a.kv_heads * k) {
-        rest -= a.kv_heads * k;
-        k = attn_key_tiles(ent, a.ratio, ++c.t, R, KT, !pass.dense);
-      }
-    } else {
-      c.t = rest / (a.kv_heads * k);
-      rest -= c.t * a.kv_heads * k;
-    }
-    c.h = rest / k;
-    c.begin = rest - c.h * k;
-    c.item = items[lo] + c.t * a.kv_heads + c.h;
+    for (int i = tid; i < pass.entities; i += kThreads) pass.plan[i] = items[i];
+  const int w0 = attn_share(tiles_before, max(min(pass.ctas, tiles_before), 1), blockIdx.x);
+  int lo = 0, hi = pass.entities;  // tiles[lo] <= w0 < tiles[hi]
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (tiles[mid] <= w0) lo = mid; else hi = mid;
   }
+  const AttnCursor c = attn_locate<R, KT>(a, pass, tiles_before, lo, w0 - tiles[lo], items[lo]);
   __syncthreads();
   return c;
 }
@@ -248,7 +280,7 @@ __device__ __forceinline__ AttnCursor attn_start(const AttnArgs& a, const AttnPa
 struct AttnSegment {
   AttnEntity ent;
   int t, h, begin, end;  // row tile, KV head, key tiles [begin, end) of `of`
-  int of, item, entity;
+  int of, item;
 };
 
 template <int R, int KT>
@@ -284,7 +316,6 @@ struct AttnWalk {
     s->end = min(k, c.begin + c.left);
     s->of = k;
     s->item = c.item;
-    s->entity = c.e;
     c.left -= s->end - s->begin;
     c.begin = 0;
     ++c.item;
@@ -293,12 +324,32 @@ struct AttnWalk {
   }
 };
 
-// What a CTA leaves for paged_join_kernel, from its last segment (any: it had one).
-__device__ __forceinline__ void attn_leave_cut(const AttnPass& pass, const AttnCursor& start, const AttnSegment& s, bool any,
-                                               int segments) {
-  const bool cut = any && s.begin == 0 && s.end < s.of;
-  reinterpret_cast<AttnCut*>(pass.plan)[blockIdx.x] = {
-      s.entity, s.t, s.h, s.end, cut ? s.of : 0, 2 * static_cast<int>(blockIdx.x) + (segments > 1), start.total, 0};
+__device__ __forceinline__ int attn_owner(int total, int ctas, int w) {
+  int c = static_cast<int>(static_cast<long long>(w) * ctas / total);
+  while (c + 1 < ctas && attn_share(total, ctas, c + 1) <= w) ++c;
+  while (c > 0 && attn_share(total, ctas, c) > w) --c;
+  return c;
+}
+
+// What a CTA leaves for paged_join_kernel: the number `segments` of its
+// segments, the last of them s.
+__device__ __forceinline__ void attn_leave_cut(const AttnArgs& a, const AttnPass& pass, const AttnCursor& start,
+                                               const AttnSegment& s, int segments, int R) {
+  AttnCut cut = {};
+  if (segments > 0 && s.begin == 0 && s.end < s.of) {
+    const int c = blockIdx.x, ctas = min(pass.ctas, start.total);
+    const int last = attn_owner(start.total, ctas, attn_share(start.total, ctas, c + 1) + s.of - s.end - 1);
+    cut = {last - c + 1, 2 * c + (segments > 1), s.t * R, s.ent.ntok * a.ratio, s.h, s.ent.tok0, 0, 0};
+  }
+  reinterpret_cast<AttnCut*>(pass.plan)[blockIdx.x] = cut;
+}
+
+// What it leaves for paged_merge_kernel: the items that it begins or ends.
+__device__ __forceinline__ void attn_leave_item(const AttnPass& pass, const AttnSegment& s) {
+  int2* items = reinterpret_cast<int2*>(pass.plan + (pass.entities + 2) / 2 * 2);
+  if (s.item >= pass.slots) return;
+  if (s.begin == 0) items[s.item].x = blockIdx.x;
+  if (s.end == s.of) items[s.item].y = blockIdx.x;
 }
 
 // Key tile k of an entity: which table, its first row there, and how many rows that table's part has.
@@ -323,12 +374,6 @@ __device__ __forceinline__ int attn_page(const AttnArgs& a, const AttnTile& tile
   if (page >= 0 && page < a.pages) return page;
   record_error(kErrBadPage);
   return a.pages;
-}
-
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
 }
 
 // TMA box (64 elements x box rows of one page and head) into a 128-byte-swizzled tile.
@@ -437,6 +482,7 @@ __global__ void __launch_bounds__(160, 2)
     s = {};
     while (!stuck && walk.next(&s)) {
       ++segments;
+      if (pass.dense && lane == 0) attn_leave_item(pass, s);
       for (int k = s.begin; k < s.end; ++k, ++n) {
         const AttnTile tile = attn_tile<KT>(s.ent, k);
         const int p = lane % per_tile, rest = lane / per_tile, half = rest % kHalves, is_v = rest / kHalves;
@@ -456,7 +502,7 @@ __global__ void __launch_bounds__(160, 2)
                       is_v ? &vmap : &kmap, half * 64, in_page, s.h, page, &full[st]);
       }
     }
-    if (!pass.dense && lane == 0) attn_leave_cut(pass, start, s, segments > 0, segments);
+    if (!pass.dense && lane == 0) attn_leave_cut(a, pass, start, s, segments, R);
     // The last copies land before the CTA's shared memory is given back.
     for (int i = max(n - C::kStages, 0); i < n; ++i)
       if (!mbar_wait_bounded(&full[i % C::kStages], (i / C::kStages) & 1)) record_error(kErrDrainTimeout);
@@ -676,61 +722,117 @@ __global__ void __launch_bounds__(160, 2)
 
 // ------------------------------------------------------------ joining segments
 
-// What a pass left of one row: its segments are those of CTAs c0..c1 at the slots below.
+// What a dense pass left of one row: segments of CTAs c0 to c1, at slots c + item.
 struct AttnRowParts {
   int c0, c1, item, row;  // c1 < c0: nothing
 };
 
-__device__ __forceinline__ int attn_owner(int total, int ctas, int w) {
-  int c = static_cast<int>(static_cast<long long>(w) * ctas / total);
-  while (c + 1 < ctas && attn_share(total, ctas, c + 1) <= w) ++c;
-  while (c > 0 && attn_share(total, ctas, c) > w) --c;
-  return c;
-}
-
 __device__ __forceinline__ AttnRowParts attn_row_parts(const AttnArgs& a, const AttnPass& pass, int e, int token, int h,
-                                                       int hr, int lane) {
+                                                       int hr) {
   AttnRowParts p = {0, -1, 0, 0};
-  const int R = pass.rows, KT = pass.keys;
+  const int before = pass.plan[e];
   const AttnEntity ent = attn_entity(a, pass.mode, e);
   const int row = (token - ent.tok0) * a.ratio + hr;
   if (row < 0 || row >= ent.ntok * a.ratio) return p;
-  const int t = row / R, k = attn_key_tiles(ent, a.ratio, t, R, KT, !pass.dense);
-  if (k == 0) return p;
-  const int total = pass.plan[pass.entities];
-  int before = 0;
-  if (ent.causal && ent.ntok > 1) {
-    for (int i = lane; i < t; i += 32) before += attn_key_tiles(ent, a.ratio, i, R, KT, !pass.dense);
-    before = warp_sum_int(before);
-  } else {
-    before = t * k;
-  }
-  const int w = pass.plan[e] + before * a.kv_heads + h * k;
-  p.row = row - t * R;
-  p.item = pass.plan[pass.entities + 1 + e] + t * a.kv_heads + h;
-  const int ctas = min(pass.ctas, total);
-  p.c0 = attn_owner(total, ctas, w);
-  p.c1 = attn_owner(total, ctas, w + k - 1);
+  const int t = row / pass.rows;
+  if (attn_key_tiles(ent, a.ratio, t, pass.rows, pass.keys, 0) == 0) return p;
+  p.row = row - t * pass.rows;
+  p.item = before + t * a.kv_heads + h;
+  if (p.item >= pass.slots) return p;
+  const int2 ctas = reinterpret_cast<const int2*>(pass.plan + (pass.entities + 2) / 2 * 2)[p.item];
+  p.c0 = max(ctas.x, 0);
+  p.c1 = min(ctas.y, pass.ctas - 1);
   return p;
 }
 
-// Adds one segment of a row into (top, sum, acc); a lane holds D / 32 consecutive elements.
+// Where a segment of a row lies (nullptr: outside the workspace).
+struct AttnSlot {
+  const float2* stats;
+  const float* acc;
+};
 template <int D>
-__device__ __forceinline__ void attn_add_segment(const AttnPass& pass, int slot, int row, int lane, float& top, float& sum,
-                                                 float (&acc)[D / 32]) {
-  constexpr int N = D / 32;
-  if (slot >= pass.slots) return;
+__device__ __forceinline__ AttnSlot attn_slot(const AttnPass& pass, int slot, int row) {
+  if (slot < 0 || slot >= pass.slots) return {nullptr, nullptr};
   const long long r = static_cast<long long>(slot) * pass.rows + row;
-  const float2 st = pass.stats[r];
-  float x[N];
-  load_values<kTypeF32, N>(pass.acc, r * D + lane * N, x);
-  const float m = fmaxf(top, st.x), z = m == -INFINITY ? 0.0f : m;
-  const float f = ex2(top - z), fx = ex2(st.x - z);
-  top = m;
-  sum = fmaf(st.y, fx, sum * f);
-#pragma unroll
-  for (int i = 0; i < N; ++i) acc[i] = fmaf(x[i], fx, acc[i] * f);
+  return {pass.stats + r, pass.acc + r * D};
 }
+
+// A row's segments joined by `parts` warps (1 or 4) of a CTA: warp `part` takes
+// every parts-th.  The lanes first read 32 segments' statistics at once (lane
+// i: segment i), so that the accumulators, D / 32 elements a lane, load
+// without waiting for one another.
+template <int D>
+struct AttnJoin {
+  static constexpr int N = D / 32;
+  float top = -INFINITY, sum = 0.0f, acc[N] = {};
+
+  // Segments i < n, i % parts == part, at row row_of(i) of slot_of(i).  Four
+  // accumulators load at a time, the first four beside the statistics.
+  template <typename At>
+  __device__ __forceinline__ void add(int n, int lane, int part, int parts, At at) {
+    for (int base = 0; base < n; base += 32 * parts) {
+      const int i = base + lane * parts + part;
+      AttnSlot mine = {nullptr, nullptr};
+      if (i < n) mine = at(i);
+      float2 st = make_float2(-INFINITY, 0.0f);
+      if (mine.stats) st = *mine.stats;
+      const int here = min((n - base - part + parts - 1) / parts, 32);
+      float x[4][N];
+      auto load = [&](int k) {
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const auto from = reinterpret_cast<const float*>(
+              __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(mine.acc), (k + u) & 31));
+#pragma unroll
+          for (int e = 0; e < N; ++e) x[u][e] = 0.0f;
+          if (k + u < here && from) load_values<kTypeF32, N>(from, lane * N, x[u]);
+        }
+      };
+      load(0);
+      const float m = fmaxf(top, warp_max_float(st.x)), z = m == -INFINITY ? 0.0f : m;
+      const float f = ex2(top - z), w = ex2(st.x - z);
+      sum = fmaf(sum, f, warp_sum_float_butterfly(st.y * w));
+      top = m;
+#pragma unroll
+      for (int e = 0; e < N; ++e) acc[e] *= f;
+      for (int k = 0; k < here; k += 4) {
+        if (k) load(k);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const float ws = __shfl_sync(0xffffffffu, w, (k + u) & 31);
+#pragma unroll
+          for (int e = 0; e < N; ++e) acc[e] = k + u < here ? fmaf(x[u][e], ws, acc[e]) : acc[e];
+        }
+      }
+    }
+  }
+
+  // The warps of a row together, in the last of them (the others return false).
+  // `shared`: 256 / 32 x (D + 2) floats.
+  __device__ __forceinline__ bool gather(float* shared, int warp, int lane, int part, int parts) {
+    if (parts == 1) return true;
+    float* mine = shared + warp * (D + 2);
+#pragma unroll
+    for (int e = 0; e < N; ++e) mine[lane * N + e] = acc[e];
+    if (lane == 0) mine[D] = top, mine[D + 1] = sum;
+    __syncthreads();
+    if (part) return false;
+    float m = top;
+    for (int p = 1; p < parts; ++p) m = fmaxf(m, mine[p * (D + 2) + D]);
+    const float z = m == -INFINITY ? 0.0f : m, f = ex2(top - z);
+    sum *= f;
+#pragma unroll
+    for (int e = 0; e < N; ++e) acc[e] *= f;
+    for (int p = 1; p < parts; ++p) {
+      const float* other = mine + p * (D + 2);
+      const float fx = ex2(other[D] - z);
+      sum = fmaf(other[D + 1], fx, sum);
+#pragma unroll
+      for (int e = 0; e < N; ++e) acc[e] = fmaf(other[lane * N + e], fx, acc[e]);
+    }
+    return true;
+  }
+};
 
 // The result of a row's segments; zeros where there was nothing to see.
 template <int D, bool kBf16>
@@ -743,55 +845,44 @@ __device__ __forceinline__ void attn_store_row(const AttnArgs& a, int token, int
   store_values16<kBf16, N>(a.out + token * a.out_token + head * a.out_head + lane * N, acc);
 }
 
-// Adds a pass's segments of one row.
-template <int D>
-__device__ __forceinline__ void attn_add_parts(const AttnPass& pass, const AttnRowParts& p, int lane, float& top,
-                                               float& sum, float (&acc)[D / 32]) {
-  for (int c = p.c0; c <= p.c1; ++c) {
-    attn_add_segment<D>(pass, c + p.item, p.row, lane, top, sum, acc);
-  }
-}
-
 // Joins the item that CTA c began and others went on with: their segments of
-// it are the first ones of their shares.  Grid (CTA c, 8 rows), a warp a row.
+// it are the first ones of their shares.  Grid (CTA c, rows of 8 / parts).
 template <int D, bool kBf16>
-__global__ void __launch_bounds__(256) paged_join_kernel(const AttnArgs a, const AttnPass pass) {
+__global__ void __launch_bounds__(256) paged_join_kernel(const AttnArgs a, const AttnPass pass, int parts) {
+  __shared__ float shared[8 * (D + 2)];
   pdl_wait_prerequisite();
   pdl_launch_dependents();
   const AttnCut cut = reinterpret_cast<const AttnCut*>(pass.plan)[blockIdx.x];
-  if (cut.of == 0) return;
-  const AttnEntity ent = attn_entity(a, pass.mode, cut.e);
-  const int lane = threadIdx.x & 31, row = blockIdx.y * 8 + (threadIdx.x >> 5), at = cut.t * pass.rows + row;
-  if (at >= ent.ntok * a.ratio) return;
-  float top = -INFINITY, sum = 0.0f, acc[D / 32];
-#pragma unroll
-  for (int i = 0; i < D / 32; ++i) acc[i] = 0.0f;
-  attn_add_segment<D>(pass, cut.slot, row, lane, top, sum, acc);
-  const int ctas = min(pass.ctas, cut.total);
-  int left = cut.of - cut.end;
-  for (int c = blockIdx.x + 1; left > 0 && c < ctas; ++c) {
-    attn_add_segment<D>(pass, 2 * c, row, lane, top, sum, acc);
-    left -= attn_share(cut.total, ctas, c + 1) - attn_share(cut.total, ctas, c);
-  }
+  if (cut.segments == 0) return;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, part = warp % parts;
+  const int row = blockIdx.y * (8 / parts) + warp / parts, at = cut.row0 + row;
+  const bool there = at < cut.rows;
+  AttnJoin<D> join;
+  if (there)
+    join.add(cut.segments, lane, part, parts,
+             [&](int i) { return attn_slot<D>(pass, i == 0 ? cut.slot : 2 * static_cast<int>(blockIdx.x + i), row); });
+  if (!join.gather(shared, warp, lane, part, parts) || !there) return;
   const int j = at / a.ratio;
-  attn_store_row<D, kBf16>(a, ent.tok0 + j, cut.h * a.ratio + at - j * a.ratio, lane, sum, acc);
+  attn_store_row<D, kBf16>(a, cut.tok0 + j, cut.h * a.ratio + at - j * a.ratio, lane, join.sum, join.acc);
 }
 
-// Prefixes apart from own rows: a warp per (token, query head) joins all
+// Prefixes apart from own rows: `parts` warps per (token, query head) join all
 // segments of both.  Rows that see nothing become zeros.  first: the prefixes'
 // pass, or the one of both; second: the own rows' pass where there are two.
 template <int D, bool kBf16>
-__global__ void __launch_bounds__(256) paged_merge_kernel(const AttnArgs a, const AttnPass first, const AttnPass second) {
+__global__ void __launch_bounds__(256)
+    paged_merge_kernel(const AttnArgs a, const AttnPass first, const AttnPass second, int parts) {
+  __shared__ float shared[8 * (D + 2)];
   pdl_wait_prerequisite();
   pdl_launch_dependents();
-  const int lane = threadIdx.x & 31, q_heads = a.kv_heads * a.ratio;
-  const long long w = static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5);
-  if (w >= static_cast<long long>(a.tokens) * q_heads) return;
-  const int token = static_cast<int>(w / q_heads), head = static_cast<int>(w % q_heads);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, part = warp % parts, q_heads = a.kv_heads * a.ratio;
+  const long long w = static_cast<long long>(blockIdx.x) * (8 / parts) + warp / parts;
+  bool there = w < static_cast<long long>(a.tokens) * q_heads;
+  const int token = there ? static_cast<int>(w / q_heads) : 0, head = static_cast<int>(w % q_heads);
   const int h = head / a.ratio, hr = head - h * a.ratio;
   int seq = token;
   if (a.q_start) {
-    if (token < a.q_start[0] || token >= a.q_start[a.seqs]) return;  // rows behind the last sequence stay
+    there = there && token >= a.q_start[0] && token < a.q_start[a.seqs];  // rows behind the last sequence stay
     int lo = 0, hi = a.seqs;
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
@@ -799,19 +890,22 @@ __global__ void __launch_bounds__(256) paged_merge_kernel(const AttnArgs a, cons
     }
     seq = lo;
   }
-  float top = -INFINITY, sum = 0.0f, acc[D / 32];
-#pragma unroll
-  for (int i = 0; i < D / 32; ++i) acc[i] = 0.0f;
-  auto add = [&](const AttnPass& pass, int e) {
-    attn_add_parts<D>(pass, attn_row_parts(a, pass, e, token, h, hr, lane), lane, top, sum, acc);
-  };
-  const int g = attn_group_of(a, seq);
-  if (g >= 0) add(first, g);
-  if (first.mode == kAttnBoth)
-    add(first, a.groups + seq);
-  else
-    add(second, seq);
-  attn_store_row<D, kBf16>(a, token, head, lane, sum, acc);
+  AttnJoin<D> join;
+  if (there) {
+    const int g = attn_group_of(a, seq);
+    AttnRowParts pre = {0, -1, 0, 0};
+    const bool both = first.mode == kAttnBoth;
+    const AttnPass& own_pass = both ? first : second;
+    const AttnRowParts own = attn_row_parts(a, own_pass, both ? a.groups + seq : seq, token, h, hr);
+    if (g >= 0) pre = attn_row_parts(a, first, g, token, h, hr);
+    const int shared_segments = pre.c1 - pre.c0 + 1;
+    join.add(shared_segments + own.c1 - own.c0 + 1, lane, part, parts, [&](int i) {
+      return i < shared_segments ? attn_slot<D>(first, pre.c0 + i + pre.item, pre.row)
+                                 : attn_slot<D>(own_pass, own.c0 + i - shared_segments + own.item, own.row);
+    });
+  }
+  if (!join.gather(shared, warp, lane, part, parts) || !there) return;
+  attn_store_row<D, kBf16>(a, token, head, lane, join.sum, join.acc);
 }
 
 }  // namespace mllb

@@ -175,6 +175,7 @@ __global__ void __launch_bounds__(384, 1)
       s = {};
       while (!stuck && walk.next(&s)) {
         ++segments;
+        if (pass.dense && lane == 0) attn_leave_item(pass, s);
         for (int k = s.begin; k < s.end && !stuck; ++k) {
           const AttnTile tile = attn_tile<KT>(s.ent, k);
           const int p = lane % per_tile, half = lane / per_tile;
@@ -198,7 +199,7 @@ __global__ void __launch_bounds__(384, 1)
           }
         }
       }
-      if (!pass.dense && lane == 0) attn_leave_cut(pass, start, s, segments > 0, segments);
+      if (!pass.dense && lane == 0) attn_leave_cut(a, pass, start, s, segments, R);
       for (int i = max(n - NS, 0); i < n; ++i)
         if (!mbar_wait_bounded(&full[i % NS], (i / NS) & 1)) record_error(kErrDrainTimeout);
     } else if (warp == 9) {

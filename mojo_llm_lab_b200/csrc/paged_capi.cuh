@@ -162,7 +162,8 @@ int paged_plan(int64_t tokens, int64_t q_heads, int64_t kv_heads, int64_t head_d
     if (slots > (1 << 30)) return fail(MLLB_EINVAL, "too many tokens x heads");
     p->slots[i] = static_cast<int>(slots);
     p->plan_off[i] = at;
-    const int64_t plan = p->dense[i] ? 2ll * (p->entities[i] + 1) * 4 : p->ctas[i] * static_cast<int64_t>(sizeof(mllb::AttnCut));
+    const int64_t plan = p->dense[i] ? (p->entities[i] + 2) / 2 * 8ll + slots * 8
+                                     : p->ctas[i] * static_cast<int64_t>(sizeof(mllb::AttnCut));
     at += (plan + 255) / 256 * 256;
     p->stats_off[i] = at;
     at += slots * p->rows[i] * 8;
@@ -230,19 +231,29 @@ int launch_attn(const mllb::AttnArgs& a, const mllb::AttnPass& pass, const CUten
   }
 }
 
+// Warps that join one row: four where the line has more CTAs than there are
+// row tiles to begin with (long contexts of few rows: tens of segments a row;
+// one sequence of 4096 rows 29 -> JOIN4 us), otherwise one.
+int join_parts(const mllb::AttnArgs& a, const mllb::AttnPass& pass) {
+  const int64_t items = static_cast<int64_t>(a.kv_heads) * ((static_cast<int64_t>(a.tokens) * a.ratio) / pass.rows + 1);
+  return items * 4 < pass.ctas ? 4 : 1;
+}
+
 template <int D>
 cudaError_t launch_join(const mllb::AttnArgs& a, const mllb::AttnPass& pass, bool bf16, cudaStream_t stream) {
   auto kernel = bf16 ? mllb::paged_join_kernel<D, true> : mllb::paged_join_kernel<D, false>;
-  return launch(kernel, dim3(static_cast<unsigned>(pass.ctas), static_cast<unsigned>(pass.rows / 8)), dim3(256), 0, stream,
-                true, a, pass);
+  const int parts = join_parts(a, pass);
+  return launch(kernel, dim3(static_cast<unsigned>(pass.ctas), static_cast<unsigned>(pass.rows * parts / 8)), dim3(256), 0,
+                stream, true, a, pass, parts);
 }
 
 template <int D>
 cudaError_t launch_merge(const mllb::AttnArgs& a, const mllb::AttnPass& p0, const mllb::AttnPass& p1, bool bf16,
                          cudaStream_t stream) {
   auto kernel = bf16 ? mllb::paged_merge_kernel<D, true> : mllb::paged_merge_kernel<D, false>;
-  const int64_t warps = static_cast<int64_t>(a.tokens) * a.kv_heads * a.ratio;
-  return launch(kernel, dim3(static_cast<unsigned>((warps + 7) / 8)), dim3(256), 0, stream, true, a, p0, p1);
+  const int parts = join_parts(a, p0);
+  const int64_t warps = static_cast<int64_t>(a.tokens) * a.kv_heads * a.ratio * parts;
+  return launch(kernel, dim3(static_cast<unsigned>((warps + 7) / 8)), dim3(256), 0, stream, true, a, p0, p1, parts);
 }
 
 }  // namespace

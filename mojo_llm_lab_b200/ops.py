@@ -25,8 +25,8 @@ import math
 import torch
 
 from . import formats as F
-from ._lib import (LAUNCH_CONST_AUX, LAUNCH_PDL, S_D_SUMQ, S_SUM_X, TYPE_BF16, TYPE_F16, TYPE_F32, ActF32,  # noqa: F401
-                   BeamRows, BeamScores, PagedAppend, PagedAttn, PagedCache, check, device_error, lib)
+from ._lib import (LAUNCH_CONST_AUX, LAUNCH_PDL, S_D_SUMQ, S_SUM_X, ActF32, check, device_error, lib,  # noqa: F401
+                   native)
 
 __all__ = [
     "quantize_q8_1", "q4_k_q8_1_matvec", "q4_k_q8_1_gate_order", "q4k_gate_up", "q6_k_q8_1_matvec",
@@ -703,10 +703,8 @@ def q5_k_q8_1_matvec(weights: torch.Tensor, activations: torch.Tensor, output: t
 #   decode_qk_rope_append / decode_attention / argmax_key for a batch: the cache
 #   is a pool of pages, a sequence is a line of a page table, sequences may share
 #   a prefix, and greedy choice becomes a selection over beams.  Lengths, rows
-#   and tables are read on the device, so a captured step follows them.
-
-_TYPE_OF = {torch.float32: TYPE_F32, torch.float16: TYPE_F16, torch.bfloat16: TYPE_BF16}
-
+#   and tables are read on the device, so a captured step follows them.  The
+#   checks and the call are native (csrc/torch_ops.cpp).
 
 def rope_frequencies(rot_dim: int, base: float = F.IMROPE_FREQ_BASE, scaling: str = "none", factor: float = 1.0,
                      original_context: int = 32768, fast_turns: float = 32.0, slow_turns: float = 1.0,
@@ -744,51 +742,6 @@ def rope_frequencies(rot_dim: int, base: float = F.IMROPE_FREQ_BASE, scaling: st
     return freqs.to(device), magnitude
 
 
-def _need_view(t: torch.Tensor, name: str, dims: int, dtypes) -> None:
-    """A CUDA tensor whose last dimension is contiguous (the others may have any stride)."""
-    if not isinstance(t, torch.Tensor):
-        raise ValueError(f"{name} must be a torch.Tensor")
-    if t.dtype not in dtypes:
-        raise ValueError(f"{name} must be one of {', '.join(map(str, dtypes))}, got {t.dtype}")
-    if t.dim() != dims:
-        raise ValueError(f"{name} must have {dims} dimensions, got {t.dim()}")
-    if t.numel() == 0:
-        raise ValueError(f"{name} is empty")
-    if t.stride(-1) != 1 and t.shape[-1] > 1:
-        raise ValueError(f"{name} must be contiguous in its last dimension")
-
-
-def _need_ints(t: torch.Tensor, name: str, shape: tuple) -> None:
-    if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or tuple(t.shape) != shape or not t.is_contiguous():
-        raise ValueError(f"{name} must be a contiguous torch.int32 tensor of shape {list(shape)}")
-
-
-def _need_cuda(*ts: torch.Tensor) -> torch.device:
-    """Every tensor on one CUDA device; checked behind shapes and types."""
-    dev = ts[0].device
-    for t in ts:
-        if t is not None and t.device != dev:
-            _same_device(*ts)
-    if dev.type != "cuda":
-        raise ValueError("the tensors must be CUDA tensors")
-    return dev
-
-
-def _paged_cache(k_cache: torch.Tensor, v_cache: torch.Tensor, layers: bool = False) -> PagedCache:
-    if layers and k_cache.dim() == 4:
-        k_cache, v_cache = k_cache.unsqueeze(0), v_cache.unsqueeze(0)
-    _need_view(k_cache, "k_cache", 5 if layers else 4, (torch.float16, torch.bfloat16))
-    if v_cache.dtype != k_cache.dtype or v_cache.shape != k_cache.shape or v_cache.stride() != k_cache.stride():
-        raise ValueError("v_cache must match k_cache in type, shape and strides")
-    shape, stride = k_cache.shape, k_cache.stride()
-    if not layers:
-        shape, stride = (1, *shape), (0, *stride)
-    # A dimension of one element may carry any stride: give it one that the kernels take.
-    page, head, row = (s if n > 1 else shape[4] * 8 for s, n in zip(stride[1:4], shape[1:4]))
-    return PagedCache(k_cache.data_ptr(), v_cache.data_ptr(), shape[1], shape[2], shape[3], shape[4], page, head, row,
-                      shape[0], stride[0], _TYPE_OF[k_cache.dtype])
-
-
 def paged_qkv_append(qkv: torch.Tensor, positions: torch.Tensor, rows: torch.Tensor, page_table: torch.Tensor,
                      k_cache: torch.Tensor, v_cache: torch.Tensor, q_heads: int, freqs: torch.Tensor,
                      seq: torch.Tensor | None = None, q_gamma: torch.Tensor | None = None,
@@ -799,37 +752,8 @@ def paged_qkv_append(qkv: torch.Tensor, positions: torch.Tensor, rows: torch.Ten
     [pages, kv_heads, page_size, head_dim].  qkv [tokens, (q_heads + 2 kv_heads) * head_dim], fp32, fp16 or bf16, rows
     of any stride; freqs as rope_frequencies gives them.  Returns q [tokens, q_heads, head_dim] in the caches' type.
     A negative rows[t] is padding: nothing is stored for it (q_out neither)."""
-    cache = _paged_cache(k_cache, v_cache)
-    _need_view(qkv, "qkv", 2, tuple(_TYPE_OF))
-    tokens, d = qkv.shape[0], cache.head_dim
-    if q_heads <= 0 or qkv.shape[1] != (q_heads + 2 * cache.kv_heads) * d:
-        raise ValueError("qkv must hold (q_heads + 2 kv_heads) x head_dim values a token")
-    _need_ints(positions, "positions", (tokens,))
-    _need_ints(rows, "rows", (tokens,))
-    if page_table.dim() != 2:
-        raise ValueError("page_table must be [sequences, pages]")
-    _need_ints(page_table, "page_table", tuple(page_table.shape))
-    if seq is not None:
-        _need_ints(seq, "seq", (tokens,))
-    elif tokens > page_table.shape[0]:
-        raise ValueError("without seq, token t is sequence t's: more tokens than sequences")
-    for name, t in (("q_gamma", q_gamma), ("k_gamma", k_gamma)):
-        if t is not None and (t.dtype != torch.float32 or t.numel() != d or not t.is_contiguous()):
-            raise ValueError(f"{name} must be {d} contiguous fp32 values")
-    if freqs.dtype != torch.float64 or freqs.dim() != 1 or not freqs.is_contiguous() or not 1 <= freqs.numel() <= d // 2:
-        raise ValueError(f"freqs must be 1 to {d // 2} contiguous fp64 values")
-    if q_out is None:
-        q_out = torch.empty(tokens, q_heads, d, dtype=k_cache.dtype, device=qkv.device)
-    elif q_out.dtype != k_cache.dtype or q_out.shape != (tokens, q_heads, d) or not q_out.is_contiguous():
-        raise ValueError("q_out must be contiguous [tokens, q_heads, head_dim] of the caches' type")
-    dev = _need_cuda(qkv, positions, rows, page_table, k_cache, v_cache, freqs, seq, q_gamma, k_gamma, q_out)
-    args = PagedAppend(qkv.data_ptr(), tokens, qkv.stride(0) if tokens > 1 else qkv.shape[1], positions.data_ptr(),
-                       rows.data_ptr(), _ptr(seq), page_table.data_ptr(), page_table.shape[0], page_table.shape[1],
-                       _ptr(q_gamma), _ptr(k_gamma), freqs.data_ptr(), 2 * freqs.numel(), q_heads, eps, magnitude,
-                       q_out.data_ptr(), _TYPE_OF[qkv.dtype], 1 if interleaved else 0)
-    with torch.cuda.device(dev):
-        check(lib().mllb_paged_qkv_append(args, cache, _flags(pdl), _stream(qkv)), "paged_qkv_append")
-    return q_out
+    return native().paged_qkv_append(qkv, positions, rows, page_table, k_cache, v_cache, q_heads, freqs, seq, q_gamma,
+                                     k_gamma, interleaved, magnitude, eps, q_out, pdl)
 
 
 def paged_attention_workspace(tokens: int, q_heads: int, kv_heads: int, head_dim: int, seqs: int, groups: int,
@@ -855,59 +779,8 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     group_start[g] .. group_start[g + 1] - 1 (None: all) see the prefix_lens[g] rows of prefix_table[g] too; these are
     read once for all of a group's sequences.  A token that sees nothing gets zeros; tokens behind q_start[-1] are left
     as they are.  scale: 1 / sqrt(head_dim) unless given."""
-    cache = _paged_cache(k_cache, v_cache)
-    _need_view(q, "q", 3, (k_cache.dtype,))
-    tokens, q_heads, d = q.shape
-    if d != cache.head_dim:
-        raise ValueError(f"q has heads of {d}, the caches of {cache.head_dim}")
-    if q_heads % cache.kv_heads:
-        raise ValueError("q_heads must be a multiple of kv_heads")
-    if page_table.dim() != 2:
-        raise ValueError("page_table must be [sequences, pages]")
-    seqs = page_table.shape[0]
-    _need_ints(page_table, "page_table", tuple(page_table.shape))
-    _need_ints(seq_lens, "seq_lens", (seqs,))
-    groups = prefix_width = 0
-    if prefix_table is not None:
-        if prefix_lens is None or prefix_table.dim() != 2:
-            raise ValueError("prefix_table must be [groups, pages] and come with prefix_lens")
-        groups, prefix_width = prefix_table.shape
-        _need_ints(prefix_table, "prefix_table", (groups, prefix_width))
-        _need_ints(prefix_lens, "prefix_lens", (groups,))
-        if group_start is not None:
-            _need_ints(group_start, "group_start", (groups + 1,))
-        elif groups > 1:
-            raise ValueError("several groups need group_start")
-    elif prefix_lens is not None or group_start is not None:
-        raise ValueError("prefix_lens and group_start need prefix_table")
-    if q_start is not None:
-        _need_ints(q_start, "q_start", (seqs + 1,))
-    elif tokens != seqs:
-        raise ValueError("without q_start every sequence has one token")
-    if out is None:
-        out = torch.empty(tokens, q_heads, d, dtype=q.dtype, device=q.device)
-    else:
-        _need_view(out, "out", 3, (q.dtype,))
-        if out.shape != q.shape:
-            raise ValueError("out must have the shape of q")
-    dev = _need_cuda(q, k_cache, v_cache, page_table, seq_lens, prefix_table, prefix_lens, group_start, q_start, out,
-                     workspace)
-    args = PagedAttn(q.data_ptr(), out.data_ptr(), tokens, q_heads, *_steps(q), *_steps(out), page_table.data_ptr(),
-                     seq_lens.data_ptr(), seqs, page_table.shape[1], _ptr(prefix_table), _ptr(prefix_lens),
-                     _ptr(group_start), groups, prefix_width, _ptr(q_start), d ** -0.5 if scale is None else scale)
-    with torch.cuda.device(dev):
-        if workspace is None:
-            workspace = paged_attention_workspace(tokens, q_heads, cache.kv_heads, d, seqs, groups, dev)
-        else:
-            _need(workspace, "workspace", torch.uint8)
-        check(lib().mllb_paged_attention(args, cache, workspace.data_ptr(), workspace.numel(), _flags(pdl), _stream(q)),
-              "paged_attention")
-    return out
-
-
-def _steps(t: torch.Tensor) -> tuple[int, int]:
-    """Strides of the first two dimensions; one of a single element counts as whole heads."""
-    return tuple(s if n > 1 else t.shape[2] for s, n in zip(t.stride()[:2], t.shape[:2]))
+    return native().paged_attention(q, k_cache, v_cache, page_table, seq_lens, prefix_table, prefix_lens, group_start,
+                                    q_start, scale, out, workspace, pdl)
 
 
 def beam_select(logits: torch.Tensor, scores: torch.Tensor, n: int | None = None, done: torch.Tensor | None = None,
@@ -919,40 +792,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, n: int | None = None
     logits [batch, beams, vocab] in fp32, fp16 or bf16, scores fp32 [batch, beams].  -inf logits are never chosen; a
     beam that is done (bool or uint8 [batch, beams]) offers only end_token at its score.  Places without a candidate
     hold -inf, -1, -1.  out: the three result tensors, to write into."""
-    _need_view(logits, "logits", 3, tuple(_TYPE_OF))
-    batch, beams, vocab = logits.shape
-    n = beams if n is None else int(n)
-    if scores.dtype != torch.float32 or scores.shape != (batch, beams) or not scores.is_contiguous():
-        raise ValueError("scores must be contiguous fp32 [batch, beams]")
-    if done is not None:
-        if done.dtype not in (torch.bool, torch.uint8) or done.shape != (batch, beams) or not done.is_contiguous():
-            raise ValueError("done must be contiguous bool or uint8 [batch, beams]")
-        if not 0 <= end_token < vocab:
-            raise ValueError("done beams need an end_token of the vocabulary")
-    need = int(lib().mllb_beam_select_workspace(batch, beams, vocab, n))
-    if need < 0:
-        check(need, "beam_select")
-    if out is None:
-        new_scores = torch.empty(batch, n, dtype=torch.float32, device=logits.device)
-        tokens, parents = torch.empty(2, batch, n, dtype=torch.int32, device=logits.device).unbind(0)
-    else:
-        new_scores, tokens, parents = out
-        if new_scores.dtype != torch.float32 or new_scores.shape != (batch, n) or not new_scores.is_contiguous():
-            raise ValueError("out scores must be contiguous fp32 [batch, n]")
-        _need_ints(tokens, "out tokens", (batch, n))
-        _need_ints(parents, "out parents", (batch, n))
-    dev = _need_cuda(logits, scores, done, new_scores, tokens, parents, workspace)
-    if workspace is None:
-        workspace = torch.empty(need, dtype=torch.uint8, device=dev)
-    else:
-        _need(workspace, "workspace", torch.uint8)
-    args = BeamScores(logits.data_ptr(), batch, beams, vocab, n, logits.stride(0) if batch > 1 else 0,
-                      logits.stride(1) if beams > 1 else 0, scores.data_ptr(), _ptr(done), end_token,
-                      _TYPE_OF[logits.dtype])
-    with torch.cuda.device(dev):
-        check(lib().mllb_beam_select(args, new_scores.data_ptr(), tokens.data_ptr(), parents.data_ptr(),
-                                     workspace.data_ptr(), workspace.numel(), _flags(pdl), _stream(logits)), "beam_select")
-    return new_scores, tokens, parents
+    return native().beam_select(logits, scores, n, done, end_token, out, workspace, pdl)
 
 
 def beam_reorder(parents: torch.Tensor, page_table: torch.Tensor, seq_lens: torch.Tensor, fresh: torch.Tensor,
@@ -963,26 +803,4 @@ def beam_reorder(parents: torch.Tensor, page_table: torch.Tensor, seq_lens: torc
     the first keeps it and each further row r gets the free page fresh[r] with the rows held so far copied (used[r] = 1)
     in the caches [pages, kv_heads, page_size, head_dim], or [layers, pages, ...] for all layers at once.  fresh pages
     are distinct and not in the table.  A negative parent ends its row (length 0).  out: the three result tensors."""
-    cache = _paged_cache(k_cache, v_cache, layers=True)
-    if parents.dim() != 2 or page_table.dim() != 2 or parents.numel() != page_table.shape[0]:
-        raise ValueError("parents must be [batch, beams] and page_table [batch * beams, pages]")
-    rows, width = page_table.shape
-    _need_ints(parents, "parents", tuple(parents.shape))
-    _need_ints(page_table, "page_table", (rows, width))
-    _need_ints(seq_lens, "seq_lens", (rows,))
-    _need_ints(fresh, "fresh", (rows,))
-    if out is None:
-        table = torch.empty_like(page_table)
-        lens, used = torch.empty(2, rows, dtype=torch.int32, device=page_table.device).unbind(0)
-    else:
-        table, lens, used = out
-        _need_ints(table, "out table", (rows, width))
-        _need_ints(lens, "out lens", (rows,))
-        _need_ints(used, "out used", (rows,))
-    dev = _need_cuda(parents, page_table, seq_lens, fresh, k_cache, v_cache, table, lens, used)
-    args = BeamRows(parents.data_ptr(), page_table.data_ptr(), seq_lens.data_ptr(), fresh.data_ptr(), parents.shape[0],
-                    parents.shape[1], width)
-    with torch.cuda.device(dev):
-        check(lib().mllb_beam_reorder(args, cache, table.data_ptr(), lens.data_ptr(), used.data_ptr(), _flags(pdl),
-                                      _stream(page_table)), "beam_reorder")
-    return table, lens, used
+    return native().beam_reorder(parents, page_table, seq_lens, fresh, k_cache, v_cache, out, pdl)
