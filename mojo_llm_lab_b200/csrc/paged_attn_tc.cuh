@@ -98,22 +98,6 @@ __device__ __forceinline__ void tc_st16(uint32_t taddr, const uint32_t* v) {
 }
 __device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// a * b + c on two fp32 values at once.
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-  float2 d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;"
-      : "=l"(reinterpret_cast<uint64_t&>(d))
-      : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)), "l"(reinterpret_cast<uint64_t&>(c)));
-  return d;
-}
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-  float2 d;
-  asm("add.rn.f32x2 %0, %1, %2;"
-      : "=l"(reinterpret_cast<uint64_t&>(d))
-      : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
-  return d;
-}
-
 template <int D, bool kBf16>
 __global__ void __launch_bounds__(384, 1)
     paged_attn_many_kernel(const AttnArgs a, const AttnPass pass, const __grid_constant__ CUtensorMap kmap,
@@ -365,15 +349,15 @@ __global__ void __launch_bounds__(384, 1)
           uint32_t p[16];
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
-            float2 w = fma2(make_float2(x[c + 2 * i], x[c + 2 * i + 1]), make_float2(scale, scale), make_float2(-z, -z));
+            float2 w = __ffma2_rn(make_float2(x[c + 2 * i], x[c + 2 * i + 1]), make_float2(scale, scale), make_float2(-z, -z));
             w.x = ex2(w.x);
             w.y = ex2(w.y);
-            part[i & 3] = add2(part[i & 3], w);
+            part[i & 3] = __fadd2_rn(part[i & 3], w);
             p[i] = pack16<kBf16>(w.x, w.y);
           }
           tc_st16(s_col + c / 2, p);
         }
-        part[0] = add2(add2(part[0], part[1]), add2(part[2], part[3]));
+        part[0] = __fadd2_rn(__fadd2_rn(part[0], part[1]), __fadd2_rn(part[2], part[3]));
         sum += part[0].x + part[0].y;
         tc_wait_st();
         tc_fence_before();

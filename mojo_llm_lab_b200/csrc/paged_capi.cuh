@@ -58,10 +58,10 @@ template <int kType>
 cudaError_t launch_scan(const mllb::BeamArgs& a, bool vector, cudaStream_t stream, bool pdl) {
   auto kernel = vector ? mllb::beam_scan_kernel<kType, true> : mllb::beam_scan_kernel<kType, false>;
   return launch(kernel, dim3(static_cast<unsigned>(a.chunks), static_cast<unsigned>(a.batch * a.beams)),
-                dim3(mllb::kBeamThreads), 0, stream, pdl, a);
+                dim3(mllb::kBeamThreads), a.steps * mllb::kBeamThreads * sizeof(float), stream, pdl, a);
 }
 
-int64_t beam_chunks(int64_t vocab) { return (vocab + mllb::kBeamChunk - 1) / mllb::kBeamChunk; }
+int64_t beam_steps(int64_t vocab) { return (vocab + mllb::kBeamStep - 1) / mllb::kBeamStep; }
 
 int check_beams(int64_t batch, int64_t beams, int64_t vocab, int64_t n) {
   if (batch <= 0 || beams <= 0 || vocab <= 0 || n <= 0) return fail(MLLB_EINVAL, "sizes must be positive");
@@ -428,7 +428,7 @@ int mllb_paged_attention(const mllb_paged_attn* p, const mllb_paged_cache* cache
 int64_t mllb_beam_select_workspace(int64_t batch, int64_t beams, int64_t vocab, int64_t n) {
   const int rc = check_beams(batch, beams, vocab, n);
   if (rc) return rc;
-  return batch * beams * beam_chunks(vocab) * (n * 8 + static_cast<int64_t>(sizeof(mllb::BeamChunkSum)));
+  return batch * beams * beam_steps(vocab) * (n * 8 + static_cast<int64_t>(sizeof(mllb::BeamChunkSum)));
 }
 
 int mllb_beam_select(const mllb_beam_scores* p, float* out_scores, int32_t* out_tokens, int32_t* out_parents,
@@ -461,7 +461,18 @@ int mllb_beam_select(const mllb_beam_scores* p, float* out_scores, int32_t* out_
   a.batch = static_cast<int>(p->batch);
   a.beams = static_cast<int>(p->beams);
   a.vocab = static_cast<int>(p->vocab);
-  a.chunks = static_cast<int>(beam_chunks(p->vocab));
+  // About four CTAs per SM (they fit at once), but no chunk shorter than a
+  // step: the fewer chunks, the less is listed and joined (256 rows of 151936
+  // bf16: chunks of 1 step BEAM1S us, of 19 BEAM19S us), while few rows want all SMs
+  // (4 rows: 38 chunks each).
+  int dev;
+  if ((rc = current_device(&dev))) return rc;
+  const int64_t steps = beam_steps(p->vocab), rows = p->batch * p->beams;
+  int64_t chunks = 4ll * sm_count(dev) / rows;
+  if (chunks < 1) chunks = 1;
+  a.steps = static_cast<int>((steps + chunks - 1) / chunks);
+  if (a.steps > mllb::kBeamStepsMost) a.steps = mllb::kBeamStepsMost;
+  a.chunks = static_cast<int>((steps + a.steps - 1) / a.steps);
   a.n = static_cast<int>(p->n);
   a.end_token = static_cast<int>(p->end_token);
   const int64_t lists = p->batch * p->beams * a.chunks;
@@ -475,7 +486,7 @@ int mllb_beam_select(const mllb_beam_scores* p, float* out_scores, int32_t* out_
                         : p->type == MLLB_TYPE_F16 ? launch_scan<mllb::kTypeF16>(a, vector, s, pdl)
                                                    : launch_scan<mllb::kTypeBf16>(a, vector, s, pdl);
   if ((rc = launched(e, "beam scan kernel"))) return rc;
-  return launched(launch(mllb::beam_pick_kernel, dim3(static_cast<unsigned>(a.batch)), dim3(mllb::kBeamThreads), 0, s, true, a),
+  return launched(launch(mllb::beam_pick_kernel, dim3(static_cast<unsigned>(a.batch)), dim3(mllb::kPickThreads), 0, s, true, a),
                   "beam pick kernel");
 }
 

@@ -118,7 +118,8 @@ def select(logits, scores, n, done, end_token):
             x = torch.where(x.isnan(), -math.inf, x.clamp(max=big))
             if not bool((x > -math.inf).any()) or not cum > -math.inf:
                 continue
-            s = cum + (x - x.logsumexp(0))
+            d = x - x.max()  # first: beside logits of 1e38 a logarithm of the sum would vanish
+            s = cum + (d - d.exp().sum().log())
             order = torch.sort(x, descending=True, stable=True).indices[:n]
             found += [(-float(s[i]), w, -float(x[i]), int(i)) for i in order if float(s[i]) > -math.inf]
         found = sorted(found)[:n]

@@ -19,8 +19,11 @@ def check(logits, scores, n, done=None, end_token=-1, device_logits=None, **kw):
     s, ref = got[0].double().cpu(), want[0]
     assert torch.equal(s.isinf(), ref.isinf())
     fine = ref.isfinite()
-    # One rounding to fp32; the sum of exponentials in fp32 terms (3 steps each), relative to 1 in the logarithm.
-    assert ((s - ref)[fine].abs() <= 2.0 ** -24 * ref[fine].abs() + 2.0 ** -22).all()
+    # One rounding to fp32, and the logarithm's error, the relative one of the sum.  A term 2^t, t = d log2(e) in fp32:
+    # the unit's 2 steps (2^-22), and t off by half a step, 2^-20 up to |t| = 32, which changes it by ln 2 times that;
+    # terms below 2^-32 are 2^-14 of the sum at most.  Equal logits have equal errors, so nothing averages out:
+    # 2^-22 + 0.7 x 2^-20 < 2^-20.
+    assert ((s - ref)[fine].abs() <= 2.0 ** -24 * ref[fine].abs() + 2.0 ** -20).all()
     return got
 
 
@@ -70,6 +73,32 @@ def test_select_first_step_and_banned_tokens():
     got = check(logits, scores, 5)
     assert got[1][0].tolist() == [2990, 2991, -1, -1, -1] and got[2][0].tolist() == [0, 0, -1, -1, -1]
     assert (got[0][0, 2:] == -math.inf).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+def test_select_masks_of_the_lowest_value(dtype):
+    """Tokens masked with the type's lowest value are candidates still: long runs of equal keys, few others among them."""
+    logits, scores = random(2, 3, 20000, dtype, 15)
+    low = torch.finfo(dtype).min
+    logits[0, 0, 40:] = low
+    logits[0, 1] = low
+    logits[0, 2, :19995] = low
+    logits[1, :, 3000:16500] = -math.inf
+    logits[1, 1, :3000] = low
+    check(logits, scores, 6)
+    check(logits, scores, 64)
+
+
+@pytest.mark.parametrize("vocab,pad", [(9000, 0), (9001, 0), (9003, 5), (40000, 8)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_select_many_rows(vocab, pad, dtype):
+    """So many rows that a CTA takes several steps of one, ending inside a step and inside a vector."""
+    logits, scores = random(150, 4, vocab, dtype, 16)
+    wide = torch.full((150, 4, vocab + pad), math.nan, dtype=dtype)
+    wide[..., :vocab] = logits
+    check(logits, scores, 5, device_logits=wide.cuda()[..., :vocab])
+    logits[..., 100:] = logits[..., 7:8]  # equal ones from there on
+    check(logits, scores, 5)
 
 
 def test_select_not_numbers():
