@@ -846,24 +846,31 @@ __device__ __forceinline__ void attn_store_row(const AttnArgs& a, int token, int
 }
 
 // Joins the item that CTA c began and others went on with: their segments of
-// it are the first ones of their shares.  Grid (CTA c, rows of 8 / parts).
+// it are the first ones of their shares.  Grid (CTA c, rows in turn); a row's
+// loads take about a microsecond, so as many warps as fit run beside one
+// another and a CTA takes several rows rather than the SMs several waves of CTAs.
 template <int D, bool kBf16>
-__global__ void __launch_bounds__(256) paged_join_kernel(const AttnArgs a, const AttnPass pass, int parts) {
+__global__ void __launch_bounds__(256, 4) paged_join_kernel(const AttnArgs a, const AttnPass pass, int parts) {
   __shared__ float shared[8 * (D + 2)];
   pdl_wait_prerequisite();
   pdl_launch_dependents();
   const AttnCut cut = reinterpret_cast<const AttnCut*>(pass.plan)[blockIdx.x];
   if (cut.segments == 0) return;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, part = warp % parts;
-  const int row = blockIdx.y * (8 / parts) + warp / parts, at = cut.row0 + row;
-  const bool there = at < cut.rows;
-  AttnJoin<D> join;
-  if (there)
-    join.add(cut.segments, lane, part, parts,
-             [&](int i) { return attn_slot<D>(pass, i == 0 ? cut.slot : 2 * static_cast<int>(blockIdx.x + i), row); });
-  if (!join.gather(shared, warp, lane, part, parts) || !there) return;
-  const int j = at / a.ratio;
-  attn_store_row<D, kBf16>(a, cut.tok0 + j, cut.h * a.ratio + at - j * a.ratio, lane, join.sum, join.acc);
+  for (int row0 = blockIdx.y * (8 / parts); row0 < pass.rows; row0 += gridDim.y * (8 / parts)) {
+    const int row = row0 + warp / parts, at = cut.row0 + row;
+    const bool there = at < cut.rows;
+    if (cut.row0 + row0 >= cut.rows) return;
+    AttnJoin<D> join;
+    if (there)
+      join.add(cut.segments, lane, part, parts,
+               [&](int i) { return attn_slot<D>(pass, i == 0 ? cut.slot : 2 * static_cast<int>(blockIdx.x + i), row); });
+    if (join.gather(shared, warp, lane, part, parts) && there) {
+      const int j = at / a.ratio;
+      attn_store_row<D, kBf16>(a, cut.tok0 + j, cut.h * a.ratio + at - j * a.ratio, lane, join.sum, join.acc);
+    }
+    if (parts > 1) __syncthreads();  // `shared` is free again
+  }
 }
 
 // Prefixes apart from own rows: `parts` warps per (token, query head) join all

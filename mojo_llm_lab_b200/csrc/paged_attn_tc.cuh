@@ -7,8 +7,9 @@
 // the same key tiles of 128:
 //   warps 0-3, 4-7  softmax of stream 0, 1: a thread is a row
 //   warp 8          TMA copies of K and V tiles into a ring
-//   warp 9          issues the matrix instructions (lane 0), owns TMEM
-//   warps 10, 11    fill the warpgroup, whose registers the softmax takes
+//   warp 9          issues the matrix instructions, owns TMEM
+//   warp 10         walks the line ahead, posts the segments, fetches their queries
+//   warp 11         fills the warpgroup, whose registers the softmax takes
 // S = Q K^T goes to 128 TMEM columns a stream; the softmax reads it, writes
 // P over it in 16 bits, and P V adds to the stream's D columns of O, with P
 // read from TMEM and V from shared memory as it lies in the cache (MN-major).
@@ -38,8 +39,10 @@ struct AttnMany {
   static constexpr int kSlots = D == 128 ? 5 : 8;
   static constexpr int kRingOff = 2 * kQTile;
   static constexpr int kBarOff = kRingOff + kSlots * kTile;
-  static constexpr int kBars = 2 * kSlots + 4 * 2 + 1;
-  static constexpr int kSmem = kBarOff + (kBars + 1) * 8;
+  static constexpr int kPosts = 2;                // segments posted ahead
+  static constexpr int kBars = 2 * kSlots + 6 * 2 + 1 + 2 * kPosts;
+  static constexpr int kPostOff = kBarOff + (kBars + 1) * 8;
+  static constexpr int kSmem = kPostOff + kPosts * static_cast<int>(sizeof(AttnSegment));
   static constexpr int kTmemCols = 512;           // S (P over it) 2 x 128, O 2 x D
   static constexpr uint32_t kSCol = 0, kOCol = 256;
   static_assert(kSmem <= 227 * 1024, "shared memory");
@@ -59,20 +62,32 @@ __host__ __device__ constexpr uint32_t attn_idesc(int n, bool b_mn_major) {
          (static_cast<uint32_t>(n >> 3) << 17) | ((128u >> 4) << 24);
 }
 
+// Matrix instruction and commit by one elected lane: all lanes of the warp call
+// them with the same operands.
 __device__ __forceinline__ void tc_mma_f16_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t add) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
+      "{\n\t.reg .pred p, e;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+      "elect.sync _|e, 0xffffffff;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
       ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(add)
       : "memory");
 }
 __device__ __forceinline__ void tc_mma_f16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t add) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
+      "{\n\t.reg .pred p, e;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+      "elect.sync _|e, 0xffffffff;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
       ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(add)
+      : "memory");
+}
+__device__ __forceinline__ void tc_commit_elected(uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\t"
+      "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}"
+      ::"r"(smem_addr(bar))
       : "memory");
 }
 
@@ -101,7 +116,8 @@ __device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sy
 template <int D, bool kBf16>
 __global__ void __launch_bounds__(384, 1)
     paged_attn_many_kernel(const AttnArgs a, const AttnPass pass, const __grid_constant__ CUtensorMap kmap,
-                           const __grid_constant__ CUtensorMap vmap) {
+                           const __grid_constant__ CUtensorMap vmap, const __grid_constant__ CUtensorMap qmap,
+                           const int q_by_tma) {
   using C = AttnMany<D>;
   constexpr int R = C::kRows, KT = C::kKeys, NS = C::kSlots;
   extern __shared__ __align__(1024) uint8_t attn_smem[];
@@ -110,26 +126,36 @@ __global__ void __launch_bounds__(384, 1)
   uint64_t* empty = full + NS;                                            // [NS] its products are done
   uint64_t* q_full = empty + NS;                                          // [2] a stream's queries are in shared memory
   uint64_t* s_full = q_full + 2;                                          // [2] its scores are in TMEM
-  uint64_t* p_full = s_full + 2;                                          // [2] its weights are, and O is at their scale
-  uint64_t* o_done = p_full + 2;                                          // [2] its products with V are done
+  uint64_t* p_full = s_full + 2;                                          // [2][2 halves] its weights are, and O is at their scale
+  uint64_t* o_done = p_full + 4;                                          // [2] its products with V are done
   uint64_t* drained = o_done + 2;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drained + 1);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  uint64_t* q_empty = drained + 1;                                        // [2] a segment's last scores are made
+  uint64_t* post_full = q_empty + 2;                                      // [kPosts] a segment is posted
+  uint64_t* post_empty = post_full + C::kPosts;                           // [kPosts] all warps have read it
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(post_empty + C::kPosts);
+  AttnSegment* posts = reinterpret_cast<AttnSegment*>(attn_smem + C::kPostOff);
+  const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x) >> 5, 0), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int i = 0; i < NS; ++i) {
       mbar_init(&full[i], 1);
       mbar_init(&empty[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&q_full[i], 128);
+      mbar_init(&q_full[i], q_by_tma ? 1 : 4);
+      mbar_init(&q_empty[i], 1);
       mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], 128);
       mbar_init(&o_done[i], 1);
+    }
+    for (int i = 0; i < 4; ++i) mbar_init(&p_full[i], 4);
+    for (int i = 0; i < C::kPosts; ++i) {
+      mbar_init(&post_full[i], 1);
+      mbar_init(&post_empty[i], 10);
     }
     mbar_init(drained, 1);
     fence_mbar_init();
     tma_prefetch_map(&kmap);
     tma_prefetch_map(&vmap);
+    tma_prefetch_map(&qmap);
   }
   if (warp == 9) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(tmem_slot)),
@@ -145,21 +171,78 @@ __global__ void __launch_bounds__(384, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  // The posted segments in their order; false behind the last (or when the
+  // walk gave up).  Every warp but the walking one takes each.
+  int post = 0;
+  auto take = [&](AttnSegment* s) {
+    const int at = post % C::kPosts;
+    if (!mbar_wait_bounded(&post_full[at], (post / C::kPosts) & 1)) {
+      record_error(kErrFullWaitTimeout);
+      return false;
+    }
+    *s = posts[at];
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&post_empty[at]);
+    ++post;
+    return s->of > 0;
+  };
   if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kOtherRegs));
-    if (warp == 8) {
+    if (warp == 10) {
+      // ------------------------------------------------ the walk along the line, ahead of the others
       AttnWalk<R, KT> walk(a, pass, start);
-      AttnSegment s;
+      AttnSegment s = {}, last = {};
+      int segments = 0, fetched[2] = {0, 0};
+      for (bool more = true; more; ++post) {
+        more = walk.next(&s);
+        if (more) {
+          ++segments;
+          last = s;
+          if (pass.dense && lane == 0) attn_leave_item(pass, s);
+        } else {
+          s.of = 0;
+        }
+        const int at = post % C::kPosts;
+        if (post >= C::kPosts && !mbar_wait_bounded(&post_empty[at], (post / C::kPosts - 1) & 1)) {
+          record_error(kErrEmptyWaitTimeout);
+          break;
+        }
+        if (lane == 0) {
+          posts[at] = s;
+          mbar_arrive(&post_full[at]);
+        }
+        __syncwarp();
+        if (!more || !q_by_tma) continue;
+        // The queries, as soon as the segment before is through with its own.
+        // Rows behind the entity's are other tokens' (or zeros): their results
+        // go nowhere.
+        for (int i = 0; i < 2; ++i) {
+          if (i && s.ent.ntok * a.ratio - s.t * R <= 128) break;
+          if (fetched[i] && !mbar_wait_bounded(&q_empty[i], (fetched[i] - 1) & 1)) {
+            record_error(kErrEmptyWaitTimeout);
+            more = false;
+            break;
+          }
+          ++fetched[i];
+          if (lane == 0) mbar_arrive_expect_tx(&q_full[i], C::kQTile);
+          __syncwarp();
+          if (lane < D / 64)
+            tma_load_4d(attn_smem + i * C::kQTile + lane * (128 * 128), &qmap, lane * 64, 0, s.h,
+                        s.ent.tok0 + (s.t * R + i * 128) / a.ratio, &q_full[i]);
+        }
+      }
+      for (int i = 0; i < 2; ++i)  // the last copies land before the CTA's shared memory is given back
+        if (fetched[i] && !mbar_wait_bounded(&q_full[i], (fetched[i] - 1) & 1)) record_error(kErrDrainTimeout);
+      if (!pass.dense && lane == 0) attn_leave_cut(a, pass, start, last, segments, R);
+    } else if (warp == 8) {
       // ------------------------------------------------ copies: K and V tiles in turn, a box a lane
+      AttnSegment s;
       const int box_rows = min(1 << a.page_shift, KT), per_tile = KT / box_rows;
       constexpr int kHalves = D / 64;
       const int boxes = per_tile * kHalves;
-      int n = 0, segments = 0;
+      int n = 0;
       bool stuck = false;
-      s = {};
-      while (!stuck && walk.next(&s)) {
-        ++segments;
-        if (pass.dense && lane == 0) attn_leave_item(pass, s);
+      while (!stuck && take(&s)) {
         for (int k = s.begin; k < s.end && !stuck; ++k) {
           const AttnTile tile = attn_tile<KT>(s.ent, k);
           const int p = lane % per_tile, half = lane / per_tile;
@@ -183,82 +266,89 @@ __global__ void __launch_bounds__(384, 1)
           }
         }
       }
-      if (!pass.dense && lane == 0) attn_leave_cut(a, pass, start, s, segments, R);
       for (int i = max(n - NS, 0); i < n; ++i)
         if (!mbar_wait_bounded(&full[i % NS], (i / NS) & 1)) record_error(kErrDrainTimeout);
     } else if (warp == 9) {
       // ------------------------------------------------ matrix instructions
-      if (lane == 0) {
-        AttnWalk<R, KT> walk(a, pass, start);
-        AttnSegment s;
-        constexpr uint32_t kQk = attn_idesc<kBf16>(KT, false), kPv = attn_idesc<kBf16>(D, true);
-        const uint32_t q_base = smem_addr(attn_smem), ring_base = smem_addr(ring);
-        int n = 0;                    // ring position of the next K tile to use
-        int qn[2] = {0, 0}, pn[2] = {0, 0};
-        bool ok = true;
-        auto wait = [&](uint64_t* bar, int phase) {
-          if (ok && !mbar_wait_bounded(bar, phase & 1)) {
-            record_error(kErrFullWaitTimeout);
-            ok = false;
-          }
-          return ok;
-        };
-        auto scores = [&](int stream, int pos) {
-          const uint32_t kt = ring_base + (pos % NS) * C::kTile, qt = q_base + stream * C::kQTile;
-#pragma unroll
-          for (int c = 0; c < D / 16; ++c) {
-            const uint32_t off = (c >> 2) * (128 * 128) + (c & 3) * 32;  // 64 elements a swizzled row, 32 bytes a step
-            tc_mma_f16_ss(tmem + C::kSCol + stream * 128, attn_desc(qt + off, 16, 1024), attn_desc(kt + off, 16, 1024), kQk,
-                          c > 0);
-          }
-          tc_commit(&s_full[stream]);
-        };
-        while (ok && walk.next(&s)) {
-          const int streams = s.ent.ntok * a.ratio - s.t * R > 128 ? 2 : 1, tiles = s.end - s.begin;
-          for (int i = 0; i < streams; ++i) wait(&q_full[i], qn[i]++);
-          wait(&full[n % NS], n / NS);
-          if (!ok) break;
-          tc_fence_after();
-          for (int i = 0; i < streams; ++i) scores(i, n);
-          tc_commit(&empty[n % NS]);
-          for (int k = 0; k < tiles; ++k, n += 2) {
-            const int vpos = n + 1, kpos = n + 2;
-            const bool more = k + 1 < tiles;
-            wait(&full[vpos % NS], vpos / NS);
-            if (more) wait(&full[kpos % NS], kpos / NS);
-            for (int i = 0; i < streams; ++i) {
-              if (!wait(&p_full[i], pn[i]++)) break;
-              tc_fence_after();
-              const uint32_t vt = ring_base + (vpos % NS) * C::kTile;
-#pragma unroll
-              for (int c = 0; c < KT / 16; ++c)
-                tc_mma_f16_ts(tmem + C::kOCol + i * 128, tmem + C::kSCol + i * 128 + c * 8,
-                              attn_desc(vt + c * 2048, KT * 128, 1024), kPv, k > 0 || c > 0);
-              tc_commit(&o_done[i]);
-              if (more) scores(i, kpos);  // over P, which the products before it have read: they run in order
-            }
-            if (!ok) break;
-            tc_commit(&empty[vpos % NS]);
-            if (more) tc_commit(&empty[kpos % NS]);
-          }
+      AttnSegment s;
+      constexpr uint32_t kQk = attn_idesc<kBf16>(KT, false), kPv = attn_idesc<kBf16>(D, true);
+      const uint64_t q_desc = attn_desc(smem_addr(attn_smem), 16, 1024), k_desc = attn_desc(smem_addr(ring), 16, 1024),
+                     v_desc = attn_desc(smem_addr(ring), KT * 128, 1024);
+      int n = 0;  // ring position of the next K tile to use
+      int qn = 0, pn = 0, qn1 = 0, pn1 = 0;
+      bool ok = true;
+      auto wait = [&](uint64_t* bar, int phase) {
+        if (ok && !mbar_wait_bounded(bar, phase & 1)) {
+          record_error(kErrFullWaitTimeout);
+          ok = false;
         }
-        // Nothing is in flight when TMEM is given back.
-        tc_commit(drained);
-        if (!mbar_wait_bounded(drained, 0)) record_error(kErrDrainTimeout);
+        ok = __all_sync(0xffffffffu, ok);
+        return ok;
+      };
+      auto scores = [&](int stream, int pos) {
+        const uint64_t qd = q_desc + stream * (C::kQTile >> 4), kd = k_desc + (pos % NS) * (C::kTile >> 4);
+#pragma unroll
+        for (int c = 0; c < D / 16; ++c) {
+          const int off = ((c >> 2) * (128 * 128) + (c & 3) * 32) >> 4;  // 64 elements a swizzled row, 32 bytes a step
+          tc_mma_f16_ss(tmem + C::kSCol + stream * 128, qd + off, kd + off, kQk, c > 0);
+        }
+        tc_commit_elected(&s_full[stream]);
+      };
+      while (ok && take(&s)) {
+        const bool both = s.ent.ntok * a.ratio - s.t * R > 128;
+        const int tiles = s.end - s.begin;
+        wait(&q_full[0], qn++);
+        if (both) wait(&q_full[1], qn1++);
+        wait(&full[n % NS], n / NS);
+        if (!ok) break;
+        tc_fence_after();
+        scores(0, n);
+        if (tiles == 1) tc_commit_elected(&q_empty[0]);
+        if (both) {
+          scores(1, n);
+          if (tiles == 1) tc_commit_elected(&q_empty[1]);
+        }
+        tc_commit_elected(&empty[n % NS]);
+        for (int k = 0; k < tiles; ++k, n += 2) {
+          const int vpos = n + 1, kpos = n + 2;
+          const bool more = k + 1 < tiles;
+          wait(&full[vpos % NS], vpos / NS);
+          if (more) wait(&full[kpos % NS], kpos / NS);
+          const uint64_t vd = v_desc + (vpos % NS) * (C::kTile >> 4);
+          auto products = [&](int stream, int phase) {
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {  // the second half's weights come while the first is multiplied
+              if (!wait(&p_full[2 * stream + half], phase)) return;
+              tc_fence_after();
+#pragma unroll
+              for (int c = half * (KT / 32); c < (half + 1) * (KT / 32); ++c)
+                tc_mma_f16_ts(tmem + C::kOCol + stream * 128, tmem + C::kSCol + stream * 128 + c * 8, vd + c * (2048 >> 4),
+                              kPv, k > 0 || c > 0);
+            }
+            tc_commit_elected(&o_done[stream]);
+            if (more) scores(stream, kpos);  // over P, which the products before it have read: they run in order
+            if (k + 2 == tiles) tc_commit_elected(&q_empty[stream]);
+          };
+          products(0, pn++);
+          if (both) products(1, pn1++);
+          if (!ok) break;
+          tc_commit_elected(&empty[vpos % NS]);
+          if (more) tc_commit_elected(&empty[kpos % NS]);
+        }
       }
+      // Nothing is in flight when TMEM is given back.
+      tc_commit_elected(drained);
+      if (!mbar_wait_bounded(drained, 0)) record_error(kErrDrainTimeout);
       __syncwarp();
     }
   } else {
     // ------------------------------------------------ softmax: this thread's row
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::kSoftmaxRegs));
-    AttnWalk<R, KT> walk(a, pass, start);
-    AttnSegment s;
     const int stream = warp >> 2, r = threadIdx.x & 127;
     const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
-    const uint32_t s_col = lanes + C::kSCol + stream * 128, o_col = lanes + C::kOCol + stream * 128;
+    const uint32_t s_col = lanes + C::kSCol + stream * 128, o_col = lanes + C::kOCol + stream * 128;  // P over S
     const float scale = fmaxf(fabsf(a.scale_log2), 1e-30f);  // q carries the sign; 0 x a masked -inf must not come up
     const uint32_t flip = a.scale_log2 < 0.0f ? 0x80008000u : 0u;
-    uint8_t* q_row = attn_smem + stream * C::kQTile + r * 128;
     int sn = 0, ring_pos = 0;
     bool first = true, stuck = false;
     auto wait = [&](uint64_t* bar, int phase) {
@@ -267,25 +357,44 @@ __global__ void __launch_bounds__(384, 1)
         stuck = true;
       }
     };
-    for (; !stuck && walk.next(&s); ring_pos += 2 * (s.end - s.begin), first = false) {
-      const int rows = s.ent.ntok * a.ratio - s.t * R;
-      if (stream && rows <= 128) continue;
-      const int row = stream * 128 + r;
-      const bool there = row < rows;
-      const int j = there ? (s.t * R + row) / a.ratio : 0;
-      const int token = s.ent.tok0 + j, head = s.h * a.ratio + (there ? s.t * R + row - j * a.ratio : 0);
-      const int limit = there ? attn_limit(s.ent, j) : 0;
-      {
-        const uint4* src = reinterpret_cast<const uint4*>(a.q + token * a.q_token + head * a.q_head);
-#pragma unroll
+    struct Row {
+      int token, head, limit;  // token -1: no such row
+    };
+    // The thread's row of a segment; its queries brought to shared memory where
+    // the copies do not (a ratio that does not divide 128, a negative scale).
+    auto load_queries = [&](const AttnSegment& s) {
+      const int at = s.t * R + stream * 128 + r;
+      const bool there = at < s.ent.ntok * a.ratio;
+      const int j = there ? at / a.ratio : 0;
+      const Row row = {there ? s.ent.tok0 + j : -1, s.h * a.ratio + (there ? at - j * a.ratio : 0),
+                       there ? attn_limit(s.ent, j) : 0};
+      if (!q_by_tma) {
+        const uint4* src = reinterpret_cast<const uint4*>(a.q + max(row.token, 0) * a.q_token + row.head * a.q_head);
+        uint8_t* dst = attn_smem + stream * C::kQTile + r * 128;
+#pragma unroll 4
         for (int c = 0; c < D / 8; ++c) {
           uint4 v = there ? src[c] : make_uint4(0, 0, 0, 0);
           v.x ^= flip, v.y ^= flip, v.z ^= flip, v.w ^= flip;
-          *reinterpret_cast<uint4*>(q_row + (c >> 3) * (128 * 128) + (((c & 7) ^ (r & 7)) << 4)) = v;
+          *reinterpret_cast<uint4*>(dst + (c >> 3) * (128 * 128) + (((c & 7) ^ (r & 7)) << 4)) = v;
         }
         fence_proxy_async_smem();
-        mbar_arrive(&q_full[stream]);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&q_full[stream]);
       }
+      return row;
+    };
+    // The next segment with rows of this stream; the tiles of those without pass by.
+    auto take_own = [&](AttnSegment* s) {
+      for (;; ring_pos += 2 * (s->end - s->begin), first = false) {
+        if (!take(s)) return false;
+        if (!stream || s->ent.ntok * a.ratio - s->t * R > 128) return true;
+      }
+    };
+    AttnSegment s;
+    Row row = {};
+    bool more = take_own(&s);
+    if (more) row = load_queries(s);
+    while (more && !stuck) {
       float top = -INFINITY, sum = 0.0f;
       for (int k = s.begin; k < s.end; ++k, ++sn) {
         const AttnTile tile = attn_tile<KT>(s.ent, k);
@@ -308,7 +417,7 @@ __global__ void __launch_bounds__(384, 1)
 #pragma unroll
         for (int c = 0; c < KT; c += 32) tc_ld32(s_col + c, x + c);
         tc_wait_ld();
-        const int end = min(tile.own ? limit : tile.rows, tile.rows) - tile.row0;
+        const int end = min(tile.own ? row.limit : tile.rows, tile.rows) - tile.row0;
         if (__any_sync(0xffffffffu, end < KT)) {
 #pragma unroll
           for (int c = 0; c < KT; ++c) x[c] = c < end ? x[c] : -INFINITY;
@@ -356,30 +465,40 @@ __global__ void __launch_bounds__(384, 1)
             p[i] = pack16<kBf16>(w.x, w.y);
           }
           tc_st16(s_col + c / 2, p);
+          if ((c + 32) % (KT / 2) == 0) {  // a half is complete
+            tc_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&p_full[2 * stream + c / (KT / 2)]);
+          }
         }
         part[0] = __fadd2_rn(__fadd2_rn(part[0], part[1]), __fadd2_rn(part[2], part[3]));
         sum += part[0].x + part[0].y;
-        tc_wait_st();
-        tc_fence_before();
-        mbar_arrive(&p_full[stream]);
       }
-      wait(&o_done[stream], sn - 1);
-      tc_fence_after();
+      // The next segment's queries can come in now (this one's last scores are
+      // made), so that its first scores are there when O has been read.
       const bool whole = s.begin == 0 && s.end == s.of;
       const bool direct = whole && !pass.dense;
       const int slot = pass.dense ? static_cast<int>(blockIdx.x) + s.item : 2 * static_cast<int>(blockIdx.x) + !first;
+      const Row mine = row;
+      ring_pos += 2 * (s.end - s.begin);
+      first = false;
+      more = take_own(&s);
+      if (more) row = load_queries(s);
+      wait(&o_done[stream], sn - 1);
+      tc_fence_after();
       const bool fits = slot < pass.slots;
       if (!direct && !fits) record_error(kErrBadPage);
       const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
-      const long long at = static_cast<long long>(slot) * R + row;
+      const long long at = static_cast<long long>(slot) * R + stream * 128 + r;
       if (!direct && fits) pass.stats[at] = make_float2(top, sum);
 #pragma unroll
       for (int c = 0; c < D; c += 32) {
         float o[32];
         tc_ld32(o_col + c, o);
         tc_wait_ld();
-        if (direct && there) {
-          uint4* dst = reinterpret_cast<uint4*>(a.out + token * a.out_token + head * a.out_head + c);
+        if (direct && mine.token >= 0) {
+          uint4* dst = reinterpret_cast<uint4*>(a.out + mine.token * a.out_token + mine.head * a.out_head + c);
 #pragma unroll
           for (int i = 0; i < 4; ++i)
             dst[i] = make_uint4(pack16<kBf16>(o[8 * i] * inv, o[8 * i + 1] * inv),

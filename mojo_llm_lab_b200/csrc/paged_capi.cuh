@@ -204,6 +204,25 @@ int registers_of(Kernel kernel) {
   return cudaFuncGetAttributes(&attr, kernel) == cudaSuccess ? attr.numRegs : 0;
 }
 
+// Row tiles of 128 queries (token, head of a KV head) x 64 elements.
+template <int D>
+int query_map(CUtensorMap* map, const mllb::AttnArgs& a, bool bf16) {
+  const EncodeTiled encode = tensor_map_encoder();
+  if (!encode) return fail(MLLB_ECUDA, "cuTensorMapEncodeTiled not found");
+  const cuuint64_t dims[4] = {D, static_cast<cuuint64_t>(a.ratio), static_cast<cuuint64_t>(a.kv_heads),
+                              static_cast<cuuint64_t>(a.tokens)};
+  const cuuint64_t strides[3] = {static_cast<cuuint64_t>(a.q_head * 2), static_cast<cuuint64_t>(a.q_head * 2 * a.ratio),
+                                 static_cast<cuuint64_t>(a.q_token * 2)};
+  const cuuint32_t box[4] = {64, static_cast<cuuint32_t>(a.ratio), 1, static_cast<cuuint32_t>(128 / a.ratio)},
+                   step[4] = {1, 1, 1, 1};
+  const CUresult r = encode(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
+                            const_cast<uint16_t*>(a.q), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(MLLB_EINVAL, "tensor map of q refused (error %d)", static_cast<int>(r));
+  return MLLB_OK;
+}
+
 template <int D>
 int launch_many(const mllb::AttnArgs& a, const mllb::AttnPass& pass, const CUtensorMap& k, const CUtensorMap& v, bool bf16,
                 int dev, cudaStream_t stream, bool pdl) {
@@ -215,8 +234,11 @@ int launch_many(const mllb::AttnArgs& a, const mllb::AttnPass& pass, const CUten
   static const int regs[2] = {registers_of(mllb::paged_attn_many_kernel<D, false>),
                               registers_of(mllb::paged_attn_many_kernel<D, true>)};
   if (regs[bf16] < C::kRegs) return fail(MLLB_ECUDA, "paged attention kernel built with %d registers", regs[bf16]);
+  CUtensorMap q = {};
+  const bool by_tma = 128 % a.ratio == 0 && a.scale_log2 >= 0.0f && a.q_head > 0 && a.q_token > 0;
+  if (by_tma && (rc = query_map<D>(&q, a, bf16))) return rc;
   return launched(launch(kernel, dim3(static_cast<unsigned>(pass.ctas)), dim3(C::kThreads), C::kSmem, stream, pdl, a, pass,
-                         k, v),
+                         k, v, by_tma ? q : k, by_tma ? 1 : 0),
                   "paged attention kernel (tensor cores)");
 }
 
@@ -243,7 +265,8 @@ template <int D>
 cudaError_t launch_join(const mllb::AttnArgs& a, const mllb::AttnPass& pass, bool bf16, cudaStream_t stream) {
   auto kernel = bf16 ? mllb::paged_join_kernel<D, true> : mllb::paged_join_kernel<D, false>;
   const int parts = join_parts(a, pass);
-  return launch(kernel, dim3(static_cast<unsigned>(pass.ctas), static_cast<unsigned>(pass.rows * parts / 8)), dim3(256), 0,
+  const int turns = pass.rows * parts / 8;
+  return launch(kernel, dim3(static_cast<unsigned>(pass.ctas), static_cast<unsigned>(parts > 1 || turns < 8 ? turns : 8)), dim3(256), 0,
                 stream, true, a, pass, parts);
 }
 

@@ -260,6 +260,24 @@ def test_attention_scales(scale):
     check_attention(c, run_attention(c, scale=scale), scale)
 
 
+@pytest.mark.parametrize("scale", [0.0, 1.0, -0.3, 1e-20])
+@pytest.mark.parametrize("hq", [8, 6])
+def test_attention_scales_of_many_tokens(scale, hq):
+    c = attention_case([300, 170], [200, 170], [100], hq=hq, spread=0.3, seed=5)
+    check_attention(c, run_attention(c, scale=scale), scale)
+
+
+def test_attention_rising_scores():
+    """Scores that grow from tile to tile, so that the running maximum has to move again and again; and huge ones."""
+    for grow in (0.02, 0.4):
+        c = attention_case([700], [120], [650], hq=4, hk=2, spread=1.0, seed=3)
+        c["q"] = c["q"].abs()
+        for lens, table in ((650, c["prefix_table"][0]), (700, c["table"][0])):
+            for at in range(lens):
+                c["kc"][int(table[at // 16]), :, at % 16] = (at if lens == 650 else 650 + at) * grow / 128
+        check_attention(c, run_attention(c))
+
+
 def test_attention_peaked_scores():
     """One key outweighs all others by far, early or late: the running maximum's corrections."""
     for at in (0, 63, 64, 500, 999):
