@@ -108,95 +108,145 @@ struct AppendArgs {
   PagedCache cache;
   long long qkv_stride;
   int tokens, q_heads, seqs, width, rot, interleaved;
-  int heads_per_cta, ctas_per_token;
+  int heads_per_warp, warps_per_token;
   float eps, magnitude;
 };
 
 constexpr int kAppendWarps = 8;
 
-// One CTA takes heads_per_cta heads of one token, a warp a head at a time; a
-// lane holds D / 32 consecutive elements.
+// A warp takes heads_per_warp heads of one token, one at a time; a lane holds
+// D / 32 consecutive elements.
 //   norm:     y = x / sqrt(sum(x^2) / D + eps) * gamma            (fp32)
 //   rotation: y'_e = y_e c_e + y_partner(e) s_e,  c = m cos, s = -+ m sin
 // The angle position * freq is taken in fp64 as turns and reduced to half a
 // turn before the fp32 sine and cosine: at position 1e6 an fp32 product would
-// be off by up to 0.06 rad.  A token's cosines and sines are the same for all
-// its heads, so a lane keeps the D / 32 pairs that its elements need.
+// be off by up to 0.06 rad.  A lane keeps the cosines and sines of its
+// elements for all its heads; warps share nothing, so none waits for another
+// (with a table made once a CTA and token, 8190 tokens of 48 heads took 86 us,
+// now APPEND_US: their CTAs were too short for their latencies).
+// Bound: HBM for prompts, one value in, one 16-bit value out; a warp has three
+// heads' loads on their way, the first before the sines are made.  One token:
+// the chain row -> page -> stores, launch latency.
 template <int D, int kType, bool kBf16>
-__global__ void __launch_bounds__(kAppendWarps * 32) paged_append_kernel(const AppendArgs a) {
-  constexpr int N = D / 32;
-  __shared__ float2 table[D / 2];
+#ifndef APMIN
+#define APMIN 4
+#endif
+#ifndef APAHEAD
+#define APAHEAD 3
+#endif
+__global__ void __launch_bounds__(kAppendWarps * 32, APMIN) paged_append_kernel(const AppendArgs a) {
+  constexpr int N = D / 32, kAhead = APAHEAD;
   __shared__ float exchange[kAppendWarps][D];
   pdl_wait_prerequisite();
   pdl_launch_dependents();
-  const int token = blockIdx.x / a.ctas_per_token;
-  const int head0 = (blockIdx.x % a.ctas_per_token) * a.heads_per_cta;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int unit = blockIdx.x * kAppendWarps + warp, token = unit / a.warps_per_token;
+  if (token >= a.tokens) return;
+  const int kv_heads = a.cache.kv_heads, heads = a.q_heads + 2 * kv_heads;
+  const int head0 = unit % a.warps_per_token * a.heads_per_warp, head1 = min(head0 + a.heads_per_warp, heads);
+  float x[kAhead][N];
+  auto load = [&](int first) {
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i)
+      if (first + i < head1) load_values<kType, N>(a.qkv, token * a.qkv_stride + (first + i) * D + lane * N, x[i]);
+  };
+  load(head0);
   const int row = a.rows[token];
   if (row < 0) return;  // padding: nothing is stored
   const int half = a.rot >> 1;
-  if (threadIdx.x < half) {
-    const double turns = a.positions[token] * (a.freqs[threadIdx.x] * 0.15915494309189533577);
-    float sn, cs;
-    sincospif(static_cast<float>(2.0 * (turns - rint(turns))), &sn, &cs);
-    table[threadIdx.x] = make_float2(cs * a.magnitude, sn * a.magnitude);
-  }
   const int seq = a.seq ? a.seq[token] : token;
   const int slot = row >> a.cache.page_shift;
   int page = -1;
   if (seq >= 0 && seq < a.seqs && slot < a.width) page = a.table[static_cast<long long>(seq) * a.width + slot];
   const bool stored = page >= 0 && page < a.cache.pages;
-  if (!stored && threadIdx.x == 0 && head0 == 0) record_error(kErrBadPage);
+  if (!stored && lane == 0 && head0 == 0) record_error(kErrBadPage);
   const long long cache_row = stored ? page * a.cache.page_stride +
                                            (row & ((1 << a.cache.page_shift) - 1)) * a.cache.row_stride : 0;
-  __syncthreads();
-
-  // This lane's cosines and signed sines, and where each element's partner is.
+  float gq[N], gk[N];
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    gq[j] = a.q_gamma ? a.q_gamma[lane * N + j] : 1.0f;
+    gk[j] = a.k_gamma ? a.k_gamma[lane * N + j] : 1.0f;
+  }
+  // Pairs lane * kPairs + q of the rotation: made here, handed round below.
+  constexpr int kPairs = D / 64;
+  float pc[kPairs], ps[kPairs];
+  const double position = a.positions[token] * 0.15915494309189533577;  // x freq: turns
+#pragma unroll
+  for (int q = 0; q < kPairs; ++q) {
+    const int pair = lane * kPairs + q;
+    const double turns = pair < half ? position * a.freqs[pair] : 0.0;
+    float sn, cs;
+    sincospif(static_cast<float>(2.0 * (turns - rint(turns))), &sn, &cs);
+    pc[q] = cs * a.magnitude;
+    ps[q] = sn * a.magnitude;
+  }
+  // This lane's cosines and signed sines, and where each element's partner is:
+  // in the lane (interleaved), at the same place of another lane (half a
+  // rotation is a whole number of lanes), or anywhere.
   float c[N], s[N];
   int partner[N];
 #pragma unroll
   for (int j = 0; j < N; ++j) {
     const int e = lane * N + j;
-    c[j] = 1.0f;
-    s[j] = 0.0f;
-    partner[j] = e;
-    if (e < a.rot) {
-      const bool second = a.interleaved ? (e & 1) : e >= half;
-      const float2 t = table[a.interleaved ? e >> 1 : (second ? e - half : e)];
-      c[j] = t.x;
-      s[j] = second ? t.y : -t.y;
-      partner[j] = a.interleaved ? e ^ 1 : (second ? e - half : e + half);
+    const bool turns = e < a.rot, second = a.interleaved ? (e & 1) : e >= half;
+    const int pair = !turns ? 0 : a.interleaved ? e >> 1 : (second ? e - half : e);
+    float cs = __shfl_sync(0xffffffffu, pc[0], pair / kPairs), sn = __shfl_sync(0xffffffffu, ps[0], pair / kPairs);
+    if constexpr (kPairs == 2) {
+      const float c1 = __shfl_sync(0xffffffffu, pc[1], pair / 2), s1 = __shfl_sync(0xffffffffu, ps[1], pair / 2);
+      if (pair & 1) cs = c1, sn = s1;
     }
+    c[j] = turns ? cs : 1.0f;
+    s[j] = !turns ? 0.0f : second ? sn : -sn;
+    partner[j] = !turns ? e : a.interleaved ? e ^ 1 : (second ? e - half : e + half);
   }
-  const int kv_heads = a.cache.kv_heads, heads = a.q_heads + 2 * kv_heads;
-  const int head1 = min(head0 + a.heads_per_cta, heads);
-  for (int head = head0 + warp; head < head1; head += kAppendWarps) {
-    float x[N];
-    load_values<kType, N>(a.qkv, token * a.qkv_stride + head * D + lane * N, x);
-    const bool is_q = head < a.q_heads, is_v = head >= a.q_heads + kv_heads;
-    if (!is_v) {
-      const float* gamma = is_q ? a.q_gamma : a.k_gamma;
-      if (gamma) {
-        float sum = 0.0f;
+  const bool by_lane = half % N == 0;
+  for (int first = head0; first < head1; first += kAhead) {
+    float y[kAhead][N];
 #pragma unroll
-        for (int j = 0; j < N; ++j) sum = fmaf(x[j], x[j], sum);
-        const float scale = rsqrtf(warp_sum_float_butterfly(sum) * (1.0f / D) + a.eps);
+    for (int i = 0; i < kAhead; ++i)
 #pragma unroll
-        for (int j = 0; j < N; ++j) x[j] = x[j] * scale * gamma[lane * N + j];
+      for (int j = 0; j < N; ++j) y[i][j] = x[i][j];
+    load(first + kAhead);
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int head = first + i;
+      if (head >= head1) break;
+      const bool is_q = head < a.q_heads, is_v = head >= a.q_heads + kv_heads;
+      if (!is_v) {
+        if (is_q ? a.q_gamma : a.k_gamma) {
+          float sum = 0.0f;
+#pragma unroll
+          for (int j = 0; j < N; ++j) sum = fmaf(y[i][j], y[i][j], sum);
+          const float scale = rsqrtf(warp_sum_float_butterfly(sum) * (1.0f / D) + a.eps);
+#pragma unroll
+          for (int j = 0; j < N; ++j) y[i][j] = y[i][j] * scale * (is_q ? gq[j] : gk[j]);
+        }
+        float other[N];
+        if (a.interleaved) {
+#pragma unroll
+          for (int j = 0; j < N; ++j) other[j] = y[i][j ^ 1];
+        } else if (by_lane) {
+#pragma unroll
+          for (int j = 0; j < N; ++j) other[j] = __shfl_sync(0xffffffffu, y[i][j], partner[j] / N);
+        } else {
+          float* ex = exchange[warp];
+          __syncwarp();
+#pragma unroll
+          for (int j = 0; j < N; ++j) ex[lane * N + j] = y[i][j];
+          __syncwarp();
+#pragma unroll
+          for (int j = 0; j < N; ++j) other[j] = ex[partner[j]];
+        }
+#pragma unroll
+        for (int j = 0; j < N; ++j) y[i][j] = fmaf(other[j], s[j], y[i][j] * c[j]);
       }
-      float* ex = exchange[warp];
-      __syncwarp();
-#pragma unroll
-      for (int j = 0; j < N; ++j) ex[lane * N + j] = x[j];
-      __syncwarp();
-#pragma unroll
-      for (int j = 0; j < N; ++j) x[j] = fmaf(ex[partner[j]], s[j], x[j] * c[j]);
-    }
-    if (is_q) {
-      store_values16<kBf16, N>(a.q_out + (static_cast<long long>(token) * a.q_heads + head) * D + lane * N, x);
-    } else if (stored) {
-      const int h = head - a.q_heads - (is_v ? kv_heads : 0);
-      store_values16<kBf16, N>((is_v ? a.cache.v : a.cache.k) + cache_row + h * a.cache.head_stride + lane * N, x);
+      if (is_q) {
+        store_values16<kBf16, N>(a.q_out + (static_cast<long long>(token) * a.q_heads + head) * D + lane * N, y[i]);
+      } else if (stored) {
+        const int h = head - a.q_heads - (is_v ? kv_heads : 0);
+        store_values16<kBf16, N>((is_v ? a.cache.v : a.cache.k) + cache_row + h * a.cache.head_stride + lane * N, y[i]);
+      }
     }
   }
 }
@@ -214,6 +264,7 @@ struct ReorderArgs {
 };
 
 constexpr int kReorderWarps = 8;
+constexpr int kReorderAhead = 8;
 
 // CTA (x, row): row's table and length come from its parent's row; the first
 // CTA writes them.  A page that is part full goes on being written by its
@@ -264,9 +315,20 @@ __global__ void __launch_bounds__(kReorderWarps * 32) beam_reorder_kernel(const 
     uint16_t* base = (kv ? a.cache.v : a.cache.k) + layer * a.cache.layer_stride + h * a.cache.head_stride;
     const uint16_t* src = base + source * a.cache.page_stride;
     uint16_t* dst = base + target * a.cache.page_stride;
-    for (int u = lane; u < part * units; u += 32) {
-      const long long at = (u / units) * a.cache.row_stride + (u % units) * 8;
-      *reinterpret_cast<uint4*>(dst + at) = *reinterpret_cast<const uint4*>(src + at);
+    // (units is 8 or 16: head_dim 64 or 128.)  Eight 16-byte loads a lane on their way.
+    const int shift = units == 16 ? 4 : 3, all = part << shift;
+    for (int u0 = lane; u0 < all; u0 += 32 * kReorderAhead) {
+      uint4 v[kReorderAhead];
+      long long at[kReorderAhead];
+#pragma unroll
+      for (int i = 0; i < kReorderAhead; ++i) {
+        const int u = u0 + 32 * i;
+        at[i] = static_cast<long long>(u >> shift) * a.cache.row_stride + (u & (units - 1)) * 8;
+        if (u < all) v[i] = *reinterpret_cast<const uint4*>(src + at[i]);
+      }
+#pragma unroll
+      for (int i = 0; i < kReorderAhead; ++i)
+        if (u0 + 32 * i < all) *reinterpret_cast<uint4*>(dst + at[i]) = v[i];
     }
   }
 }

@@ -328,14 +328,12 @@ int mllb_paged_qkv_append(const mllb_paged_append* p, const mllb_paged_cache* ca
   a.magnitude = static_cast<float>(p->magnitude);
   int dev;
   if ((rc = current_device(&dev))) return rc;
-  // One head a warp while that leaves the SMs with at most four CTAs each
-  // (latency); beyond it a CTA takes the whole token, so that its cosines and
-  // sines are made once.
-  const int64_t spread = (heads + mllb::kAppendWarps - 1) / mllb::kAppendWarps;
-  const bool few = p->tokens * spread <= 4ll * sm_count(dev);
-  a.heads_per_cta = few ? mllb::kAppendWarps : static_cast<int>(heads);
-  a.ctas_per_token = few ? static_cast<int>(spread) : 1;
-  const unsigned grid = static_cast<unsigned>(p->tokens * a.ctas_per_token);
+  // One head a warp while all warps fit at once (latency); beyond it half a
+  // token's heads a warp, so that the sines are made twice a token only.
+  const bool few = p->tokens * heads <= 32ll * sm_count(dev);
+  a.heads_per_warp = few ? 1 : static_cast<int>((heads + 1) / 2);
+  a.warps_per_token = static_cast<int>((heads + a.heads_per_warp - 1) / a.heads_per_warp);
+  const unsigned grid = static_cast<unsigned>((p->tokens * a.warps_per_token + mllb::kAppendWarps - 1) / mllb::kAppendWarps);
   const bool bf16 = cache->type == MLLB_TYPE_BF16, pdl = flags & MLLB_LAUNCH_PDL;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   cudaError_t e;
