@@ -516,7 +516,9 @@ int mllb_argmax_f32(const float *x, int64_t n, int64_t index_offset, int64_t *ke
  * rows, and beam search's selection and reordering.  Table entries, lengths
  * and rows are read on the device (a captured graph follows them); one that
  * lies outside its table or cache sets device error bit 8 (mask 0x100) and
- * reads or writes nothing through it.
+ * reads or writes nothing through it.  MLLB_LAUNCH_PDL is accepted and changes
+ * nothing: these kernels are always scheduled early, and wait for the
+ * preceding kernel before they read or write anything.
  * ---------------------------------------------------------------------- */
 
 #define MLLB_TYPE_F32 0

@@ -123,19 +123,13 @@ constexpr int kAppendWarps = 8;
 // be off by up to 0.06 rad.  A lane keeps the cosines and sines of its
 // elements for all its heads; warps share nothing, so none waits for another
 // (with a table made once a CTA and token, 8190 tokens of 48 heads took 86 us,
-// now APPEND_US: their CTAs were too short for their latencies).
-// Bound: HBM for prompts, one value in, one 16-bit value out; a warp has three
+// now 60: those CTAs were too short for their latencies).
+// Bound: HBM for prompts, one value in, one 16-bit value out; a warp has two
 // heads' loads on their way, the first before the sines are made.  One token:
 // the chain row -> page -> stores, launch latency.
 template <int D, int kType, bool kBf16>
-#ifndef APMIN
-#define APMIN 4
-#endif
-#ifndef APAHEAD
-#define APAHEAD 3
-#endif
-__global__ void __launch_bounds__(kAppendWarps * 32, APMIN) paged_append_kernel(const AppendArgs a) {
-  constexpr int N = D / 32, kAhead = APAHEAD;
+__global__ void __launch_bounds__(kAppendWarps * 32, 4) paged_append_kernel(const AppendArgs a) {
+  constexpr int N = D / 32, kAhead = 2;
   __shared__ float exchange[kAppendWarps][D];
   pdl_wait_prerequisite();
   pdl_launch_dependents();

@@ -59,17 +59,20 @@ struct AttnPass {
   int slots;       // capacity of the workspace
   int rows, keys;  // R and KT of the kernel that ran it (for the merge)
   // For the kernel that joins.  dense: [entities] items before each entity,
-  // then int2 [items] first and last CTA of an item; otherwise [ctas] AttnCut.
+  // then int2 [items] first and last CTA of an item; otherwise AttnCut, the
+  // number of records first (as segments), then one an item (by_item: there are
+  // no more items than CTAs) or one a CTA.
   int32_t* plan;
+  int by_item;
   float* acc;      // [slots][R][D]
   float2* stats;   // [slots][R] (maximum in powers of two, sum)
 };
 
-// The item that CTA c began and others went on with (segments 0: none): how
-// many segments, the slot of CTA c's, the item's first row of its entity's
+// An item that CTA `cta` began and others went on with (segments 0: none): how
+// many segments, the slot of that CTA's, the item's first row of its entity's
 // `rows`, its KV head and the entity's first token.
 struct AttnCut {
-  int segments, slot, row0, rows, h, tok0, pad0, pad1;
+  int segments, slot, row0, rows, h, tok0, cta, pad;
 };
 
 struct AttnEntity {
@@ -207,8 +210,8 @@ __device__ __forceinline__ AttnCursor attn_locate(const AttnArgs& a, const AttnP
 }
 
 // Adds up all entities' work and finds this CTA's share.  All threads of the
-// CTA call it; `scan` is shared scratch of 2 (entities + 1) + 64 ints.  For a
-// dense pass CTA 0 leaves the numbers of items in pass.plan.
+// CTA call it; `scan` is shared scratch of 2 (entities + 1) + 64 ints.  CTA 0
+// leaves the numbers of items, or of records, in pass.plan.
 template <int R, int KT, int kThreads>
 __device__ __forceinline__ AttnCursor attn_start(const AttnArgs& a, const AttnPass& pass, int* scan) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -223,7 +226,10 @@ __device__ __forceinline__ AttnCursor attn_start(const AttnArgs& a, const AttnPa
       const int wu = __shfl_up_sync(0xffffffffu, ws, d), nu = __shfl_up_sync(0xffffffffu, ns, d);
       if (lane >= d) ws += wu, ns += nu;
     }
-    if (blockIdx.x == 0 && pass.dense && warp == 0 && lane < pass.entities) pass.plan[lane] = ns - n;
+    if (blockIdx.x == 0 && warp == 0) {
+      if (!pass.dense && lane == 31) pass.plan[0] = pass.by_item ? ns : pass.ctas;
+      if (pass.dense && lane < pass.entities) pass.plan[lane] = ns - n;
+    }
     const int total = __shfl_sync(0xffffffffu, ws, 31), ctas = min(pass.ctas, total);
     const int w0 = attn_share(total, max(ctas, 1), blockIdx.x);
     // The entity that holds pair w0: the first whose sum passes it.
@@ -263,8 +269,11 @@ __device__ __forceinline__ AttnCursor attn_start(const AttnArgs& a, const AttnPa
     items[pass.entities] = items_before;
   }
   __syncthreads();
-  if (blockIdx.x == 0 && pass.dense)
-    for (int i = tid; i < pass.entities; i += kThreads) pass.plan[i] = items[i];
+  if (blockIdx.x == 0) {
+    if (!pass.dense && tid == 0) pass.plan[0] = pass.by_item ? items_before : pass.ctas;
+    if (pass.dense)
+      for (int i = tid; i < pass.entities; i += kThreads) pass.plan[i] = items[i];
+  }
   const int w0 = attn_share(tiles_before, max(min(pass.ctas, tiles_before), 1), blockIdx.x);
   int lo = 0, hi = pass.entities;  // tiles[lo] <= w0 < tiles[hi]
   while (hi - lo > 1) {
@@ -331,17 +340,20 @@ __device__ __forceinline__ int attn_owner(int total, int ctas, int w) {
   return c;
 }
 
-// What a CTA leaves for paged_join_kernel: the number `segments` of its
-// segments, the last of them s.
+// What a CTA leaves for paged_join_kernel behind segment s, its `segments`-th
+// (last: there is none behind it).  An item's first CTA writes the item's
+// record; by CTA, each writes one, of its last segment.
 __device__ __forceinline__ void attn_leave_cut(const AttnArgs& a, const AttnPass& pass, const AttnCursor& start,
-                                               const AttnSegment& s, int segments, int R) {
+                                               const AttnSegment& s, int segments, bool last, int R) {
+  const bool begins = segments > 0 && s.begin == 0;
+  if (pass.by_item ? !begins || s.item >= pass.ctas : !last) return;
   AttnCut cut = {};
-  if (segments > 0 && s.begin == 0 && s.end < s.of) {
+  if (begins && s.end < s.of) {
     const int c = blockIdx.x, ctas = min(pass.ctas, start.total);
-    const int last = attn_owner(start.total, ctas, attn_share(start.total, ctas, c + 1) + s.of - s.end - 1);
-    cut = {last - c + 1, 2 * c + (segments > 1), s.t * R, s.ent.ntok * a.ratio, s.h, s.ent.tok0, 0, 0};
+    const int end = attn_owner(start.total, ctas, attn_share(start.total, ctas, c + 1) + s.of - s.end - 1);
+    cut = {end - c + 1, 2 * c + (segments > 1), s.t * R, s.ent.ntok * a.ratio, s.h, s.ent.tok0, c, 0};
   }
-  reinterpret_cast<AttnCut*>(pass.plan)[blockIdx.x] = cut;
+  reinterpret_cast<AttnCut*>(pass.plan)[1 + (pass.by_item ? s.item : static_cast<int>(blockIdx.x))] = cut;
 }
 
 // What it leaves for paged_merge_kernel: the items that it begins or ends.
@@ -482,7 +494,12 @@ __global__ void __launch_bounds__(160, 2)
     s = {};
     while (!stuck && walk.next(&s)) {
       ++segments;
-      if (pass.dense && lane == 0) attn_leave_item(pass, s);
+      if (lane == 0) {
+        if (pass.dense)
+          attn_leave_item(pass, s);
+        else if (pass.by_item)
+          attn_leave_cut(a, pass, start, s, segments, false, R);
+      }
       for (int k = s.begin; k < s.end; ++k, ++n) {
         const AttnTile tile = attn_tile<KT>(s.ent, k);
         const int p = lane % per_tile, rest = lane / per_tile, half = rest % kHalves, is_v = rest / kHalves;
@@ -502,7 +519,7 @@ __global__ void __launch_bounds__(160, 2)
                       is_v ? &vmap : &kmap, half * 64, in_page, s.h, page, &full[st]);
       }
     }
-    if (!pass.dense && lane == 0) attn_leave_cut(a, pass, start, s, segments, R);
+    if (!pass.dense && !pass.by_item && lane == 0) attn_leave_cut(a, pass, start, s, segments, true, R);
     // The last copies land before the CTA's shared memory is given back.
     for (int i = max(n - C::kStages, 0); i < n; ++i)
       if (!mbar_wait_bounded(&full[i % C::kStages], (i / C::kStages) & 1)) record_error(kErrDrainTimeout);
@@ -845,8 +862,8 @@ __device__ __forceinline__ void attn_store_row(const AttnArgs& a, int token, int
   store_values16<kBf16, N>(a.out + token * a.out_token + head * a.out_head + lane * N, acc);
 }
 
-// Joins the item that CTA c began and others went on with: their segments of
-// it are the first ones of their shares.  Grid (CTA c, rows in turn); a row's
+// Joins an item that one CTA began and others went on with: their segments of
+// it are the first ones of their shares.  Grid (record, rows in turn); a row's
 // loads take about a microsecond, so as many warps as fit run beside one
 // another and a CTA takes several rows rather than the SMs several waves of CTAs.
 template <int D, bool kBf16>
@@ -854,8 +871,8 @@ __global__ void __launch_bounds__(256, 4) paged_join_kernel(const AttnArgs a, co
   __shared__ float shared[8 * (D + 2)];
   pdl_wait_prerequisite();
   pdl_launch_dependents();
-  const AttnCut cut = reinterpret_cast<const AttnCut*>(pass.plan)[blockIdx.x];
-  if (cut.segments == 0) return;
+  const AttnCut cut = reinterpret_cast<const AttnCut*>(pass.plan)[1 + blockIdx.x];
+  if (static_cast<int>(blockIdx.x) >= pass.plan[0] || cut.segments == 0) return;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, part = warp % parts;
   for (int row0 = blockIdx.y * (8 / parts); row0 < pass.rows; row0 += gridDim.y * (8 / parts)) {
     const int row = row0 + warp / parts, at = cut.row0 + row;
@@ -864,7 +881,7 @@ __global__ void __launch_bounds__(256, 4) paged_join_kernel(const AttnArgs a, co
     AttnJoin<D> join;
     if (there)
       join.add(cut.segments, lane, part, parts,
-               [&](int i) { return attn_slot<D>(pass, i == 0 ? cut.slot : 2 * static_cast<int>(blockIdx.x + i), row); });
+               [&](int i) { return attn_slot<D>(pass, i == 0 ? cut.slot : 2 * (cut.cta + i), row); });
     if (join.gather(shared, warp, lane, part, parts) && there) {
       const int j = at / a.ratio;
       attn_store_row<D, kBf16>(a, cut.tok0 + j, cut.h * a.ratio + at - j * a.ratio, lane, join.sum, join.acc);

@@ -198,7 +198,12 @@ __global__ void __launch_bounds__(384, 1)
         if (more) {
           ++segments;
           last = s;
-          if (pass.dense && lane == 0) attn_leave_item(pass, s);
+          if (lane == 0) {
+            if (pass.dense)
+              attn_leave_item(pass, s);
+            else if (pass.by_item)
+              attn_leave_cut(a, pass, start, s, segments, false, R);
+          }
         } else {
           s.of = 0;
         }
@@ -233,7 +238,7 @@ __global__ void __launch_bounds__(384, 1)
       }
       for (int i = 0; i < 2; ++i)  // the last copies land before the CTA's shared memory is given back
         if (fetched[i] && !mbar_wait_bounded(&q_full[i], (fetched[i] - 1) & 1)) record_error(kErrDrainTimeout);
-      if (!pass.dense && lane == 0) attn_leave_cut(a, pass, start, last, segments, R);
+      if (!pass.dense && !pass.by_item && lane == 0) attn_leave_cut(a, pass, start, last, segments, true, R);
     } else if (warp == 8) {
       // ------------------------------------------------ copies: K and V tiles in turn, a box a lane
       AttnSegment s;

@@ -10,6 +10,11 @@
 
 namespace {
 
+// All launches here carry the programmatic-serialisation attribute: the kernels
+// touch global memory only behind griddepcontrol.wait, so they may always be
+// scheduled while the preceding kernel runs (MLLB_LAUNCH_PDL changes nothing).
+constexpr bool kEarly = true;
+
 int log2_exact(int64_t n) {
   int s = 0;
   while ((1ll << s) < n) ++s;
@@ -49,16 +54,16 @@ int paged_cache(const mllb_paged_cache* c, mllb::PagedCache* out) {
 }
 
 template <int D, int kType>
-cudaError_t launch_append(const mllb::AppendArgs& a, bool bf16, unsigned grid, cudaStream_t stream, bool pdl) {
+cudaError_t launch_append(const mllb::AppendArgs& a, bool bf16, unsigned grid, cudaStream_t stream) {
   auto kernel = bf16 ? mllb::paged_append_kernel<D, kType, true> : mllb::paged_append_kernel<D, kType, false>;
-  return launch(kernel, dim3(grid), dim3(mllb::kAppendWarps * 32), 0, stream, pdl, a);
+  return launch(kernel, dim3(grid), dim3(mllb::kAppendWarps * 32), 0, stream, kEarly, a);
 }
 
 template <int kType>
-cudaError_t launch_scan(const mllb::BeamArgs& a, bool vector, cudaStream_t stream, bool pdl) {
+cudaError_t launch_scan(const mllb::BeamArgs& a, bool vector, cudaStream_t stream) {
   auto kernel = vector ? mllb::beam_scan_kernel<kType, true> : mllb::beam_scan_kernel<kType, false>;
   return launch(kernel, dim3(static_cast<unsigned>(a.chunks), static_cast<unsigned>(a.batch * a.beams)),
-                dim3(mllb::kBeamThreads), a.steps * mllb::kBeamThreads * sizeof(float), stream, pdl, a);
+                dim3(mllb::kBeamThreads), a.steps * mllb::kBeamThreads * sizeof(float), stream, kEarly, a);
 }
 
 int64_t beam_steps(int64_t vocab) { return (vocab + mllb::kBeamStep - 1) / mllb::kBeamStep; }
@@ -109,7 +114,7 @@ int paged_map(CUtensorMap* map, const mllb_paged_cache* c, void* base, int box_r
 // workspace query and in the call.
 struct PagedPlan {
   int passes;
-  int mode[2], rows[2], keys[2], ctas[2], entities[2], slots[2], dense[2];
+  int mode[2], rows[2], keys[2], ctas[2], entities[2], slots[2], dense[2], by_item[2], records[2];
   int64_t plan_off[2], stats_off[2], acc_off[2], bytes;
 };
 
@@ -158,12 +163,14 @@ int paged_plan(int64_t tokens, int64_t q_heads, int64_t kv_heads, int64_t head_d
     // Items: every entity's last row tile may be part full.
     const int64_t covers = p->mode[i] == mllb::kAttnBoth && groups ? 2 : 1;
     const int64_t items = kv_heads * (covers * ((tokens * ratio + p->rows[i] - 1) / p->rows[i]) + p->entities[i]);
+    p->by_item[i] = !p->dense[i] && items <= p->ctas[i];
+    p->records[i] = p->by_item[i] ? static_cast<int>(items) : p->ctas[i];
     const int64_t slots = p->dense[i] ? p->ctas[i] + items : 2 * p->ctas[i];
     if (slots > (1 << 30)) return fail(MLLB_EINVAL, "too many tokens x heads");
     p->slots[i] = static_cast<int>(slots);
     p->plan_off[i] = at;
     const int64_t plan = p->dense[i] ? (p->entities[i] + 2) / 2 * 8ll + slots * 8
-                                     : p->ctas[i] * static_cast<int64_t>(sizeof(mllb::AttnCut));
+                                     : (p->ctas[i] + 1) * static_cast<int64_t>(sizeof(mllb::AttnCut));
     at += (plan + 255) / 256 * 256;
     p->stats_off[i] = at;
     at += slots * p->rows[i] * 8;
@@ -188,12 +195,12 @@ int check_attn_sizes(int64_t tokens, int64_t q_heads, int64_t kv_heads, int64_t 
 
 template <int D, int R>
 int launch_few(const mllb::AttnArgs& a, const mllb::AttnPass& pass, const CUtensorMap& k, const CUtensorMap& v, bool bf16,
-               int dev, cudaStream_t stream, bool pdl) {
+               int dev, cudaStream_t stream) {
   using C = mllb::AttnFew<D, R>;
   auto kernel = bf16 ? mllb::paged_attn_few_kernel<D, R, true> : mllb::paged_attn_few_kernel<D, R, false>;
   int grid, per_sm, rc;
   if ((rc = stream_grid(kernel, C::kSmem, C::kThreads, dev, pass.ctas, &grid, &per_sm))) return rc;
-  return launched(launch(kernel, dim3(static_cast<unsigned>(pass.ctas)), dim3(C::kThreads), C::kSmem, stream, pdl, a, pass,
+  return launched(launch(kernel, dim3(static_cast<unsigned>(pass.ctas)), dim3(C::kThreads), C::kSmem, stream, kEarly, a, pass,
                          k, v),
                   "paged attention kernel");
 }
@@ -225,7 +232,7 @@ int query_map(CUtensorMap* map, const mllb::AttnArgs& a, bool bf16) {
 
 template <int D>
 int launch_many(const mllb::AttnArgs& a, const mllb::AttnPass& pass, const CUtensorMap& k, const CUtensorMap& v, bool bf16,
-                int dev, cudaStream_t stream, bool pdl) {
+                int dev, cudaStream_t stream) {
   using C = mllb::AttnMany<D>;
   auto kernel = bf16 ? mllb::paged_attn_many_kernel<D, true> : mllb::paged_attn_many_kernel<D, false>;
   int grid, per_sm, rc;
@@ -237,19 +244,19 @@ int launch_many(const mllb::AttnArgs& a, const mllb::AttnPass& pass, const CUten
   CUtensorMap q = {};
   const bool by_tma = 128 % a.ratio == 0 && a.scale_log2 >= 0.0f && a.q_head > 0 && a.q_token > 0;
   if (by_tma && (rc = query_map<D>(&q, a, bf16))) return rc;
-  return launched(launch(kernel, dim3(static_cast<unsigned>(pass.ctas)), dim3(C::kThreads), C::kSmem, stream, pdl, a, pass,
+  return launched(launch(kernel, dim3(static_cast<unsigned>(pass.ctas)), dim3(C::kThreads), C::kSmem, stream, kEarly, a, pass,
                          k, v, by_tma ? q : k, by_tma ? 1 : 0),
                   "paged attention kernel (tensor cores)");
 }
 
 template <int D>
 int launch_attn(const mllb::AttnArgs& a, const mllb::AttnPass& pass, const CUtensorMap& k, const CUtensorMap& v, bool bf16,
-                int dev, cudaStream_t stream, bool pdl) {
+                int dev, cudaStream_t stream) {
   switch (pass.rows) {
-    case 16: return launch_few<D, 16>(a, pass, k, v, bf16, dev, stream, pdl);
-    case 32: return launch_few<D, 32>(a, pass, k, v, bf16, dev, stream, pdl);
-    case 64: return launch_few<D, 64>(a, pass, k, v, bf16, dev, stream, pdl);
-    default: return launch_many<D>(a, pass, k, v, bf16, dev, stream, pdl);
+    case 16: return launch_few<D, 16>(a, pass, k, v, bf16, dev, stream);
+    case 32: return launch_few<D, 32>(a, pass, k, v, bf16, dev, stream);
+    case 64: return launch_few<D, 64>(a, pass, k, v, bf16, dev, stream);
+    default: return launch_many<D>(a, pass, k, v, bf16, dev, stream);
   }
 }
 
@@ -262,12 +269,12 @@ int join_parts(const mllb::AttnArgs& a, const mllb::AttnPass& pass) {
 }
 
 template <int D>
-cudaError_t launch_join(const mllb::AttnArgs& a, const mllb::AttnPass& pass, bool bf16, cudaStream_t stream) {
+cudaError_t launch_join(const mllb::AttnArgs& a, const mllb::AttnPass& pass, int records, bool bf16, cudaStream_t stream) {
   auto kernel = bf16 ? mllb::paged_join_kernel<D, true> : mllb::paged_join_kernel<D, false>;
   const int parts = join_parts(a, pass);
   const int turns = pass.rows * parts / 8;
-  return launch(kernel, dim3(static_cast<unsigned>(pass.ctas), static_cast<unsigned>(parts > 1 || turns < 8 ? turns : 8)), dim3(256), 0,
-                stream, true, a, pass, parts);
+  return launch(kernel, dim3(static_cast<unsigned>(records), static_cast<unsigned>(parts > 1 || turns < 8 ? turns : 8)), dim3(256), 0,
+                stream, kEarly, a, pass, parts);
 }
 
 template <int D>
@@ -276,7 +283,7 @@ cudaError_t launch_merge(const mllb::AttnArgs& a, const mllb::AttnPass& p0, cons
   auto kernel = bf16 ? mllb::paged_merge_kernel<D, true> : mllb::paged_merge_kernel<D, false>;
   const int parts = join_parts(a, p0);
   const int64_t warps = static_cast<int64_t>(a.tokens) * a.kv_heads * a.ratio * parts;
-  return launch(kernel, dim3(static_cast<unsigned>((warps + 7) / 8)), dim3(256), 0, stream, true, a, p0, p1, parts);
+  return launch(kernel, dim3(static_cast<unsigned>((warps + 7) / 8)), dim3(256), 0, stream, kEarly, a, p0, p1, parts);
 }
 
 }  // namespace
@@ -334,17 +341,17 @@ int mllb_paged_qkv_append(const mllb_paged_append* p, const mllb_paged_cache* ca
   a.heads_per_warp = few ? 1 : static_cast<int>((heads + 1) / 2);
   a.warps_per_token = static_cast<int>((heads + a.heads_per_warp - 1) / a.heads_per_warp);
   const unsigned grid = static_cast<unsigned>((p->tokens * a.warps_per_token + mllb::kAppendWarps - 1) / mllb::kAppendWarps);
-  const bool bf16 = cache->type == MLLB_TYPE_BF16, pdl = flags & MLLB_LAUNCH_PDL;
+  const bool bf16 = cache->type == MLLB_TYPE_BF16;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   cudaError_t e;
   if (d == 128)
-    e = p->qkv_type == MLLB_TYPE_F32   ? launch_append<128, mllb::kTypeF32>(a, bf16, grid, s, pdl)
-        : p->qkv_type == MLLB_TYPE_F16 ? launch_append<128, mllb::kTypeF16>(a, bf16, grid, s, pdl)
-                                       : launch_append<128, mllb::kTypeBf16>(a, bf16, grid, s, pdl);
+    e = p->qkv_type == MLLB_TYPE_F32   ? launch_append<128, mllb::kTypeF32>(a, bf16, grid, s)
+        : p->qkv_type == MLLB_TYPE_F16 ? launch_append<128, mllb::kTypeF16>(a, bf16, grid, s)
+                                       : launch_append<128, mllb::kTypeBf16>(a, bf16, grid, s);
   else
-    e = p->qkv_type == MLLB_TYPE_F32   ? launch_append<64, mllb::kTypeF32>(a, bf16, grid, s, pdl)
-        : p->qkv_type == MLLB_TYPE_F16 ? launch_append<64, mllb::kTypeF16>(a, bf16, grid, s, pdl)
-                                       : launch_append<64, mllb::kTypeBf16>(a, bf16, grid, s, pdl);
+    e = p->qkv_type == MLLB_TYPE_F32   ? launch_append<64, mllb::kTypeF32>(a, bf16, grid, s)
+        : p->qkv_type == MLLB_TYPE_F16 ? launch_append<64, mllb::kTypeF16>(a, bf16, grid, s)
+                                       : launch_append<64, mllb::kTypeBf16>(a, bf16, grid, s);
   return launched(e, "paged append kernel");
 }
 
@@ -422,6 +429,7 @@ int mllb_paged_attention(const mllb_paged_attn* p, const mllb_paged_cache* cache
     pass[i].entities = plan.entities[i];
     pass[i].ctas = plan.ctas[i];
     pass[i].dense = plan.dense[i];
+    pass[i].by_item = plan.by_item[i];
     pass[i].slots = plan.slots[i];
     pass[i].rows = plan.rows[i];
     pass[i].keys = plan.keys[i];
@@ -433,13 +441,13 @@ int mllb_paged_attention(const mllb_paged_attn* p, const mllb_paged_cache* cache
     CUtensorMap kmap, vmap;
     const int box = static_cast<int>(cache->page_size < plan.keys[i] ? cache->page_size : plan.keys[i]);
     if ((rc = paged_map(&kmap, cache, cache->k, box)) || (rc = paged_map(&vmap, cache, cache->v, box))) return rc;
-    const bool pdl = i > 0 || (flags & MLLB_LAUNCH_PDL);
-    rc = cache->head_dim == 128 ? launch_attn<128>(a, pass[i], kmap, vmap, bf16, dev, s, pdl)
-                                : launch_attn<64>(a, pass[i], kmap, vmap, bf16, dev, s, pdl);
+    rc = cache->head_dim == 128 ? launch_attn<128>(a, pass[i], kmap, vmap, bf16, dev, s)
+                                : launch_attn<64>(a, pass[i], kmap, vmap, bf16, dev, s);
     if (rc) return rc;
   }
   if (!pass[0].dense)
-    return launched(cache->head_dim == 128 ? launch_join<128>(a, pass[0], bf16, s) : launch_join<64>(a, pass[0], bf16, s),
+    return launched(cache->head_dim == 128 ? launch_join<128>(a, pass[0], plan.records[0], bf16, s)
+                                           : launch_join<64>(a, pass[0], plan.records[0], bf16, s),
                     "paged join kernel");
   return launched(cache->head_dim == 128 ? launch_merge<128>(a, pass[0], pass[1], bf16, s)
                                          : launch_merge<64>(a, pass[0], pass[1], bf16, s),
@@ -502,12 +510,11 @@ int mllb_beam_select(const mllb_beam_scores* p, float* out_scores, int32_t* out_
   // 16-byte loads where every row starts on that boundary.
   const bool vector = aligned(p->logits, 16) && (p->batch_stride * size) % 16 == 0 && (p->beam_stride * size) % 16 == 0;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const bool pdl = flags & MLLB_LAUNCH_PDL;
-  const cudaError_t e = p->type == MLLB_TYPE_F32   ? launch_scan<mllb::kTypeF32>(a, vector, s, pdl)
-                        : p->type == MLLB_TYPE_F16 ? launch_scan<mllb::kTypeF16>(a, vector, s, pdl)
-                                                   : launch_scan<mllb::kTypeBf16>(a, vector, s, pdl);
+  const cudaError_t e = p->type == MLLB_TYPE_F32   ? launch_scan<mllb::kTypeF32>(a, vector, s)
+                        : p->type == MLLB_TYPE_F16 ? launch_scan<mllb::kTypeF16>(a, vector, s)
+                                                   : launch_scan<mllb::kTypeBf16>(a, vector, s);
   if ((rc = launched(e, "beam scan kernel"))) return rc;
-  return launched(launch(mllb::beam_pick_kernel, dim3(static_cast<unsigned>(a.batch)), dim3(mllb::kPickThreads), 0, s, true, a),
+  return launched(launch(mllb::beam_pick_kernel, dim3(static_cast<unsigned>(a.batch)), dim3(mllb::kPickThreads), 0, s, kEarly, a),
                   "beam pick kernel");
 }
 
@@ -546,7 +553,7 @@ int mllb_beam_reorder(const mllb_beam_rows* p, const mllb_paged_cache* cache, in
   const int64_t triples = 2 * cache->layers * cache->kv_heads;
   const int64_t ctas = (triples + mllb::kReorderWarps - 1) / mllb::kReorderWarps;
   return launched(launch(mllb::beam_reorder_kernel, dim3(static_cast<unsigned>(ctas), static_cast<unsigned>(rows)),
-                         dim3(mllb::kReorderWarps * 32), 0, static_cast<cudaStream_t>(stream), flags & MLLB_LAUNCH_PDL, a),
+                         dim3(mllb::kReorderWarps * 32), 0, static_cast<cudaStream_t>(stream), kEarly, a),
                   "beam reorder kernel");
 }
 
