@@ -880,11 +880,11 @@ __global__ void __launch_bounds__(256, 4) paged_join_kernel(const AttnArgs a, co
     if (cut.row0 + row0 >= cut.rows) return;
     AttnJoin<D> join;
     if (there)
-      join.add(cut.segments, lane, part, parts,
+      join.add(min(cut.segments, pass.ctas), lane, part, parts,
                [&](int i) { return attn_slot<D>(pass, i == 0 ? cut.slot : 2 * (cut.cta + i), row); });
     if (join.gather(shared, warp, lane, part, parts) && there) {
       const int j = at / a.ratio;
-      attn_store_row<D, kBf16>(a, cut.tok0 + j, cut.h * a.ratio + at - j * a.ratio, lane, join.sum, join.acc);
+      if (cut.tok0 + j < a.tokens) attn_store_row<D, kBf16>(a, cut.tok0 + j, cut.h * a.ratio + at - j * a.ratio, lane, join.sum, join.acc);
     }
     if (parts > 1) __syncthreads();  // `shared` is free again
   }

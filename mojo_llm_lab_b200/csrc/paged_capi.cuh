@@ -124,19 +124,33 @@ int tile_rows(int64_t rows) {
   return rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : mllb::AttnMany<128>::kRows;
 }
 
+// Whether every sequence reads its group's prefix for itself although few rows
+// each do so: the prefixes come from L2 after the first time, and one pass has
+// less to join and to launch.  By the bytes read again at most, as the tables'
+// widths bound them: 64 MB against a pass of prefixes and own rows (fp16, heads
+// of 128, own rows 100; 16 sequences of a 1000-row prefix, 60 MB, 18.5 us
+// against 19.4; of 4000, 236 MB, 32.8 against 24.5), 192 MB against a pass each
+// (40 of 1000, 156 MB, 28.3 against 36.9; of 4000, 614 MB, 63 against 41.6).
+bool prefix_repeats(const mllb_paged_attn* p, const mllb_paged_cache* c) {
+  const int64_t again = (p->seqs - p->groups) * p->prefix_width * c->page_size * c->kv_heads * c->head_dim * 4;
+  const bool together = p->groups && (p->tokens * (p->q_heads / c->kv_heads) + p->groups - 1) / p->groups <= 64;
+  return p->groups && again <= (together ? 64ll : 192ll) << 20;
+}
+
 // Mean query rows (tokens x query heads of a KV head) of a sequence and of a
 // group decide the shape.  A sequence with a row tile's worth of rows shares
 // nothing more by going through its group, so prefix and own rows then run as
-// one softmax (no segments to join); with few rows a sequence, the prefix
-// runs once a group.
-int paged_plan(int64_t tokens, int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t seqs, int64_t groups, int dev,
-              PagedPlan* p) {
+// one softmax (no segments to join); so they do where `repeat` says.  Otherwise
+// the prefix runs once a group: in one pass with the own rows where a group's
+// rows fit one tile, in a pass of its own on the tensor cores beyond.
+int paged_plan(int64_t tokens, int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t seqs, int64_t groups,
+               bool repeat, int dev, PagedPlan* p) {
   const int64_t ratio = q_heads / kv_heads;
   const int64_t seq_rows = (tokens * ratio + seqs - 1) / seqs;
   const int64_t group_rows = groups ? (tokens * ratio + groups - 1) / groups : 0;
   memset(p, 0, sizeof(*p));
   p->passes = 1;
-  if (groups == 0 || groups >= seqs || seq_rows >= 64) {
+  if (groups == 0 || groups >= seqs || seq_rows >= 64 || repeat) {
     p->mode[0] = groups ? mllb::kAttnConcat : mllb::kAttnOwn;
     p->rows[0] = tile_rows(seq_rows);
     p->entities[0] = static_cast<int>(seqs);
@@ -360,9 +374,10 @@ int64_t mllb_paged_attention_workspace(int64_t tokens, int64_t q_heads, int64_t 
   int dev, rc;
   if ((rc = check_attn_sizes(tokens, q_heads, kv_heads, head_dim, seqs, groups))) return rc;
   if ((rc = current_device(&dev))) return rc;
-  PagedPlan plan;
-  if ((rc = paged_plan(tokens, q_heads, kv_heads, head_dim, seqs, groups, dev, &plan))) return rc;
-  return plan.bytes;
+  PagedPlan plan, other;  // which of them a call takes depends on its page tables, too
+  if ((rc = paged_plan(tokens, q_heads, kv_heads, head_dim, seqs, groups, false, dev, &plan))) return rc;
+  if ((rc = paged_plan(tokens, q_heads, kv_heads, head_dim, seqs, groups, true, dev, &other))) return rc;
+  return plan.bytes > other.bytes ? plan.bytes : other.bytes;
 }
 
 int mllb_paged_attention(const mllb_paged_attn* p, const mllb_paged_cache* cache, void* workspace, int64_t workspace_bytes,
@@ -389,7 +404,9 @@ int mllb_paged_attention(const mllb_paged_attn* p, const mllb_paged_cache* cache
   int dev;
   if ((rc = current_device(&dev))) return rc;
   PagedPlan plan;
-  if ((rc = paged_plan(p->tokens, p->q_heads, cache->kv_heads, cache->head_dim, p->seqs, p->groups, dev, &plan))) return rc;
+  const bool repeat = prefix_repeats(p, cache);
+  if ((rc = paged_plan(p->tokens, p->q_heads, cache->kv_heads, cache->head_dim, p->seqs, p->groups, repeat, dev, &plan)))
+    return rc;
   if (workspace_bytes < plan.bytes)
     return fail(MLLB_EINVAL, "workspace of %lld bytes, %lld needed", static_cast<long long>(workspace_bytes),
                 static_cast<long long>(plan.bytes));

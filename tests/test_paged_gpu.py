@@ -137,7 +137,9 @@ def test_append_rows_without_a_page_store_nothing():
 # ------------------------------------------------------------------ attention
 
 def attention_case(lens, news=None, prefix=(), group_start=None, hq=8, hk=2, d=128, page=16, dtype=F16, seed=0,
-                   rows_first=False, spread=2.0):
+                   rows_first=False, spread=2.0, apart=True):
+    """apart: the prefixes' table is so wide (behind its pages stand numbers that are never read) that prefixes run
+    once a group; else a call of this size has every sequence read its prefix again."""
     g = torch.Generator().manual_seed(seed)
     news = [1] * len(lens) if news is None else news
     starts = [0]
@@ -158,6 +160,11 @@ def attention_case(lens, news=None, prefix=(), group_start=None, hq=8, hk=2, d=1
         c["prefix_table"] = table[b:, :max(1, -(-max(prefix) // page))].contiguous()
         c["prefix_lens"] = list(prefix)
         c["group_start"] = [0, b] if group_start is None else group_start
+        if apart and b > len(prefix):
+            columns = 192 * 2 ** 20 // ((b - len(prefix)) * page * hk * d * 4) + 1
+            wide = torch.full((len(prefix), max(columns, c["prefix_table"].shape[1])), 2 ** 31 - 1, dtype=torch.int32)
+            wide[:, :c["prefix_table"].shape[1]] = c["prefix_table"]
+            c["prefix_table"] = wide
     return c
 
 
@@ -206,9 +213,10 @@ def test_attention_pages(page, rows_first, d):
     (12, [200, 90], [2, 5, 9], 4, 1), (7, [50, 60, 70], [0, 3, 3, 7], 4, 1), (3, [40, 50, 60], [0, 1, 2, 3], 4, 2),
     (150, [1025], None, 10, 2)])
 @pytest.mark.parametrize("dtype", [F16, BF16])
-def test_attention_shared_prefixes(seqs, prefix, group_start, hq, hk, dtype):
+@pytest.mark.parametrize("apart", [True, False])
+def test_attention_shared_prefixes(seqs, prefix, group_start, hq, hk, dtype, apart):
     lens = [(37 * i) % 150 for i in range(seqs)]
-    c = attention_case(lens, prefix=prefix, group_start=group_start, hq=hq, hk=hk, seed=seqs, dtype=dtype)
+    c = attention_case(lens, prefix=prefix, group_start=group_start, hq=hq, hk=hk, seed=seqs, dtype=dtype, apart=apart)
     check_attention(c, run_attention(c))
 
 
@@ -219,9 +227,9 @@ def test_attention_shared_prefixes(seqs, prefix, group_start, hq, hk, dtype):
     ([4, 0, 6], [9, 3, 6], [33], 4, 2, 128),        # ... or the prefix alone
     ([200, 150, 90], [64, 2, 90], [500], 8, 2, 128), ([600, 550], [600, 400], [333], 8, 2, 128),
     ([64, 64, 64, 64], [4, 4, 3, 2], [1000], 8, 2, 128), ([1100], [1030], [129], 2, 1, 64)])
-@pytest.mark.parametrize("dtype", [F16, BF16])
-def test_attention_many_tokens(lens, news, prefix, hq, hk, d, dtype):
-    c = attention_case(lens, news, prefix, hq=hq, hk=hk, d=d, dtype=dtype, seed=sum(lens))
+@pytest.mark.parametrize("dtype,apart", [(F16, True), (BF16, True), (F16, False)])
+def test_attention_many_tokens(lens, news, prefix, hq, hk, d, dtype, apart):
+    c = attention_case(lens, news, prefix, hq=hq, hk=hk, d=d, dtype=dtype, seed=sum(lens), apart=apart)
     check_attention(c, run_attention(c))
 
 
@@ -287,8 +295,9 @@ def test_attention_peaked_scores():
         check_attention(c, run_attention(c))
 
 
-def test_attention_bad_pages_are_flagged_and_stay_inside():
-    c = attention_case([200, 100, 64], prefix=[80], seed=8)
+@pytest.mark.parametrize("apart", [True, False])
+def test_attention_bad_pages_are_flagged_and_stay_inside(apart):
+    c = attention_case([200, 100, 64], prefix=[80], seed=8, apart=apart)
     good = run_attention(c).cpu()
     c["table"][0, 3], c["table"][0, 5] = -5, c["kc"].shape[0]
     out = run_attention(c)
@@ -303,8 +312,9 @@ def test_attention_bad_pages_are_flagged_and_stay_inside():
     assert ops.device_error() == BAD_PAGE
 
 
-def test_attention_starts_that_make_no_sense_stay_inside():
-    c = attention_case([90, 200, 30], [3, 70, 5], [64], seed=22)
+@pytest.mark.parametrize("apart", [True, False])
+def test_attention_starts_that_make_no_sense_stay_inside(apart):
+    c = attention_case([90, 200, 30], [3, 70, 5], [64], seed=22, apart=apart)
     c["starts"] = [0, 10 ** 6, -3, 78]
     c["group_start"] = [7, -2]
     run_attention(c)
@@ -349,10 +359,10 @@ def test_attention_on_another_stream_and_twice_at_once():
     check_attention(b, outs[1])
 
 
-@pytest.mark.parametrize("prefix", [[], [150]])
-def test_captured_attention_follows_lengths(prefix):
+@pytest.mark.parametrize("prefix,apart", [([], False), ([150], False), ([150], True)])
+def test_captured_attention_follows_lengths(prefix, apart):
     """One captured launch, replayed while the lengths grow across tiles and pages."""
-    c = attention_case([200, 180, 140], prefix=prefix, seed=31)
+    c = attention_case([200, 180, 140], prefix=prefix, seed=31, apart=apart)
     q, kc, vc, table = c["q"].cuda(), P.to_dev(c["kc"].nan_to_num()), P.to_dev(c["vc"].nan_to_num()), c["table"].cuda()
     c["kc"], c["vc"] = kc.cpu(), vc.cpu()
     lens = torch.tensor([1, 1, 1], dtype=torch.int32).cuda()
