@@ -2,9 +2,10 @@
 // entry, the n of highest score
 //   score[w][v] = cum[w] + x[w][v] - log(sum over u of exp(x[w][u])),
 // ties to the lower beam, in a beam to the larger logit (far below the beam's
-// best, fp64 scores of different logits meet), then to the lower token.  Within a beam the order is that of the
-// logits, so one pass over them finds both the n best of every chunk and the
-// chunk's part of the sum; a second, small kernel joins them in fp64.
+// best, fp64 scores of different logits meet), then to the lower token.  Within
+// a beam the order is that of the logits, so one pass over them finds both the n
+// best of every chunk and the chunk's part of the sum; a second, small kernel
+// joins them in fp64.
 //
 // Logits: NaN counts as -inf, +inf as the largest finite fp32, and -inf is
 // no candidate (nor is anything of a beam whose cum is -inf or NaN).
@@ -171,7 +172,9 @@ __device__ __forceinline__ void beam_best(BeamScratch& sh, int total, int n, uns
 // Key of a logit: its ordered bits above the complement of its index; 0 is no
 // candidate.  Bound: issue slots, about 8 a logit (unpack, NaN, maximum,
 // difference, product, ex2, sum), rather than its 2 or 4 bytes from HBM, and
-// for short chunks the latencies of the selection.
+// for short chunks the latencies of the selection.  Both kernels, 32 x 8 rows of
+// 151936 in bf16: n = 8 33 us, n = 16 with a quarter of the beams done 39; the
+// bytes alone 12.  4 rows in fp32: 11.
 template <int kType, bool kVector>
 __global__ void __launch_bounds__(kBeamThreads, 4) beam_scan_kernel(const BeamArgs a) {
   constexpr int kWide = kVector ? (kType == kTypeF32 ? 4 : 8) : 1;  // values of one load

@@ -120,6 +120,10 @@ struct PagedPlan {
 
 // Row tile for entities of `rows` query rows: up to 64 the kernel for few rows
 // a key, in its narrowest shape that holds them; beyond, the tensor cores'.
+// 48 sequences of 4000 rows, 8 KV heads: 4 rows 101 us (in tiles of 32: 105), 32
+// rows 110 us (in tiles of 64: 168).  33 to 64 rows lie between: 48 sequences
+// of 16 tokens on 200 rows take 29 us (the other kernel's starts and ends: 33),
+// on 2000 rows 102 us (91).
 int tile_rows(int64_t rows) {
   return rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : mllb::AttnMany<128>::kRows;
 }
@@ -141,8 +145,10 @@ bool prefix_repeats(const mllb_paged_attn* p, const mllb_paged_cache* c) {
 // group decide the shape.  A sequence with a row tile's worth of rows shares
 // nothing more by going through its group, so prefix and own rows then run as
 // one softmax (no segments to join); so they do where `repeat` says.  Otherwise
-// the prefix runs once a group: in one pass with the own rows where a group's
-// rows fit one tile, in a pass of its own on the tensor cores beyond.
+// the prefix runs once a group (16 sequences over a prefix of 8000 rows: 32 rows
+// each 55 us, as one softmax 142; 128 rows each 109 us, as one softmax 112): in
+// one pass with the own rows where a group's rows fit one tile, in a pass of its
+// own on the tensor cores beyond.
 int paged_plan(int64_t tokens, int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t seqs, int64_t groups,
                bool repeat, int dev, PagedPlan* p) {
   const int64_t ratio = q_heads / kv_heads;
@@ -274,18 +280,19 @@ int launch_attn(const mllb::AttnArgs& a, const mllb::AttnPass& pass, const CUten
   }
 }
 
-// Warps that join one row: four where the line has more CTAs than there are
-// row tiles to begin with (long contexts of few rows: tens of segments a row;
-// one sequence of 4096 rows 29 -> JOIN4 us), otherwise one.
-int join_parts(const mllb::AttnArgs& a, const mllb::AttnPass& pass) {
-  const int64_t items = static_cast<int64_t>(a.kv_heads) * ((static_cast<int64_t>(a.tokens) * a.ratio) / pass.rows + 1);
-  return items * 4 < pass.ctas ? 4 : 1;
+// Warps that join one row: four while all rows' fit on the SMs at once (few rows
+// of long contexts have tens of segments each; one sequence of 4096 rows 12.4 us,
+// with one warp a row 17.5), otherwise one, which has less to gather (16
+// sequences of up to 8 tokens over a prefix of 8000 rows 55 us, with four 68).
+int join_parts(const mllb::AttnArgs& a, int dev) {
+  return static_cast<int64_t>(a.tokens) * a.kv_heads * a.ratio * 4 <= 32ll * sm_count(dev) ? 4 : 1;
 }
 
 template <int D>
-cudaError_t launch_join(const mllb::AttnArgs& a, const mllb::AttnPass& pass, int records, bool bf16, cudaStream_t stream) {
+cudaError_t launch_join(const mllb::AttnArgs& a, const mllb::AttnPass& pass, int records, bool bf16, int dev,
+                        cudaStream_t stream) {
   auto kernel = bf16 ? mllb::paged_join_kernel<D, true> : mllb::paged_join_kernel<D, false>;
-  const int parts = join_parts(a, pass);
+  const int parts = join_parts(a, dev);
   const int turns = pass.rows * parts / 8;
   return launch(kernel, dim3(static_cast<unsigned>(records), static_cast<unsigned>(parts > 1 || turns < 8 ? turns : 8)), dim3(256), 0,
                 stream, kEarly, a, pass, parts);
@@ -293,9 +300,9 @@ cudaError_t launch_join(const mllb::AttnArgs& a, const mllb::AttnPass& pass, int
 
 template <int D>
 cudaError_t launch_merge(const mllb::AttnArgs& a, const mllb::AttnPass& p0, const mllb::AttnPass& p1, bool bf16,
-                         cudaStream_t stream) {
+                         int dev, cudaStream_t stream) {
   auto kernel = bf16 ? mllb::paged_merge_kernel<D, true> : mllb::paged_merge_kernel<D, false>;
-  const int parts = join_parts(a, p0);
+  const int parts = join_parts(a, dev);
   const int64_t warps = static_cast<int64_t>(a.tokens) * a.kv_heads * a.ratio * parts;
   return launch(kernel, dim3(static_cast<unsigned>((warps + 7) / 8)), dim3(256), 0, stream, kEarly, a, p0, p1, parts);
 }
@@ -349,10 +356,12 @@ int mllb_paged_qkv_append(const mllb_paged_append* p, const mllb_paged_cache* ca
   a.magnitude = static_cast<float>(p->magnitude);
   int dev;
   if ((rc = current_device(&dev))) return rc;
-  // One head a warp while all warps fit at once (latency); beyond it half a
-  // token's heads a warp, so that the sines are made twice a token only.
-  const bool few = p->tokens * heads <= 32ll * sm_count(dev);
-  a.heads_per_warp = few ? 1 : static_cast<int>((heads + 1) / 2);
+  // As many warps a token as run at once with all others (one head each: 77
+  // tokens of 48 heads 4.4 us, half a token's each 10.3; 1024 tokens 11.1 us,
+  // one head each 30.8), two at least: each makes the token's sines again.
+  int64_t warps = 32ll * sm_count(dev) / p->tokens;
+  warps = warps < 2 ? 2 : warps > heads ? heads : warps;
+  a.heads_per_warp = static_cast<int>((heads + warps - 1) / warps);
   a.warps_per_token = static_cast<int>((heads + a.heads_per_warp - 1) / a.heads_per_warp);
   const unsigned grid = static_cast<unsigned>((p->tokens * a.warps_per_token + mllb::kAppendWarps - 1) / mllb::kAppendWarps);
   const bool bf16 = cache->type == MLLB_TYPE_BF16;
@@ -463,11 +472,11 @@ int mllb_paged_attention(const mllb_paged_attn* p, const mllb_paged_cache* cache
     if (rc) return rc;
   }
   if (!pass[0].dense)
-    return launched(cache->head_dim == 128 ? launch_join<128>(a, pass[0], plan.records[0], bf16, s)
-                                           : launch_join<64>(a, pass[0], plan.records[0], bf16, s),
+    return launched(cache->head_dim == 128 ? launch_join<128>(a, pass[0], plan.records[0], bf16, dev, s)
+                                           : launch_join<64>(a, pass[0], plan.records[0], bf16, dev, s),
                     "paged join kernel");
-  return launched(cache->head_dim == 128 ? launch_merge<128>(a, pass[0], pass[1], bf16, s)
-                                         : launch_merge<64>(a, pass[0], pass[1], bf16, s),
+  return launched(cache->head_dim == 128 ? launch_merge<128>(a, pass[0], pass[1], bf16, dev, s)
+                                         : launch_merge<64>(a, pass[0], pass[1], bf16, dev, s),
                   "paged merge kernel");
 }
 
@@ -508,9 +517,9 @@ int mllb_beam_select(const mllb_beam_scores* p, float* out_scores, int32_t* out_
   a.beams = static_cast<int>(p->beams);
   a.vocab = static_cast<int>(p->vocab);
   // About four CTAs per SM (they fit at once), but no chunk shorter than a
-  // step: the fewer chunks, the less is listed and joined (256 rows of 151936
-  // bf16: chunks of 1 step BEAM1S us, of 19 BEAM19S us), while few rows want all SMs
-  // (4 rows: 38 chunks each).
+  // step: the fewer chunks, the less is listed and joined (32 x 8 rows of 151936
+  // bf16: 33 us, in chunks of one step 81), while few rows want all SMs (1 x 4:
+  // 11 us, with one CTA for 36 steps of a row 23).
   int dev;
   if ((rc = current_device(&dev))) return rc;
   const int64_t steps = beam_steps(p->vocab), rows = p->batch * p->beams;
