@@ -127,6 +127,26 @@ __device__ __forceinline__ void tc_st16(uint32_t taddr, const uint32_t* v) {
 }
 __device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// Eight 16-byte pieces of this lane's row -> piece `lane % 8` of the rows of the
+// eight lanes around it, so that a store covers 128 bytes of four rows and not
+// 16 of 32.
+__device__ __forceinline__ void transpose8(uint4 (&v)[8], int lane) {
+#pragma unroll
+  for (int d = 1; d < 8; d <<= 1) {
+    const bool upper = lane & d;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      if (j & d) continue;
+      uint4 give = upper ? v[j] : v[j | d];
+      give.x = __shfl_xor_sync(0xffffffffu, give.x, d);
+      give.y = __shfl_xor_sync(0xffffffffu, give.y, d);
+      give.z = __shfl_xor_sync(0xffffffffu, give.z, d);
+      give.w = __shfl_xor_sync(0xffffffffu, give.w, d);
+      if (upper) v[j] = give; else v[j | d] = give;
+    }
+  }
+}
+
 template <int D, bool kBf16>
 __global__ void __launch_bounds__(384, 1)
     paged_attn_many_kernel(const AttnArgs a, const AttnPass pass, const __grid_constant__ CUtensorMap kmap,
@@ -511,23 +531,49 @@ __global__ void __launch_bounds__(384, 1)
       const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
       const long long at = static_cast<long long>(slot) * R + stream * 128 + r;
       if (keeps) pass.stats[at] = make_float2(top, sum);
+      const int near = lane & ~7, piece = lane & 7;
+      if (direct) {
+        const long long place = mine.token * a.out_token + mine.head * a.out_head;
+#pragma unroll 1
+        for (int c = 0; c < D; c += 64) {
+          uint4 v[8];
 #pragma unroll
-      for (int c = 0; c < D; c += 32) {
-        float o[32];
-        tc_ld32(o_col + c, o);
-        tc_wait_ld();
-        if (direct && mine.token >= 0) {
-          uint4* dst = reinterpret_cast<uint4*>(a.out + mine.token * a.out_token + mine.head * a.out_head + c);
+          for (int h = 0; h < 2; ++h) {
+            float o[32];
+            tc_ld32(o_col + c + 32 * h, o);
+            tc_wait_ld();
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            dst[i] = make_uint4(pack16<kBf16>(o[8 * i] * inv, o[8 * i + 1] * inv),
-                                pack16<kBf16>(o[8 * i + 2] * inv, o[8 * i + 3] * inv),
-                                pack16<kBf16>(o[8 * i + 4] * inv, o[8 * i + 5] * inv),
-                                pack16<kBf16>(o[8 * i + 6] * inv, o[8 * i + 7] * inv));
-        } else if (keeps) {
-          float4* dst = reinterpret_cast<float4*>(pass.acc + at * D + c);
+            for (int i = 0; i < 4; ++i)
+              v[4 * h + i] = make_uint4(pack16<kBf16>(o[8 * i] * inv, o[8 * i + 1] * inv),
+                                        pack16<kBf16>(o[8 * i + 2] * inv, o[8 * i + 3] * inv),
+                                        pack16<kBf16>(o[8 * i + 4] * inv, o[8 * i + 5] * inv),
+                                        pack16<kBf16>(o[8 * i + 6] * inv, o[8 * i + 7] * inv));
+          }
+          transpose8(v, lane);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) dst[i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+          for (int i = 0; i < 8; ++i) {
+            const long long to = __shfl_sync(0xffffffffu, place, near + i);
+            const bool there = __shfl_sync(0xffffffffu, mine.token, near + i) >= 0;
+            if (there) *reinterpret_cast<uint4*>(a.out + to + c + piece * 8) = v[i];
+          }
+        }
+      } else if (fits) {
+        float* row0 = pass.acc + (at - lane + near) * D + piece * 4;
+        const unsigned rows = __ballot_sync(0xffffffffu, keeps) >> near;
+#pragma unroll 1
+        for (int c = 0; c < D; c += 32) {
+          float o[32];
+          tc_ld32(o_col + c, o);
+          tc_wait_ld();
+          uint4 v[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            v[i] = make_uint4(__float_as_uint(o[4 * i]), __float_as_uint(o[4 * i + 1]), __float_as_uint(o[4 * i + 2]),
+                              __float_as_uint(o[4 * i + 3]));
+          transpose8(v, lane);
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (rows >> i & 1) *reinterpret_cast<uint4*>(row0 + i * D + c) = v[i];
         }
       }
       tc_fence_before();  // the next item's products write O
