@@ -118,60 +118,76 @@ struct PagedPlan {
   int64_t plan_off[2], stats_off[2], acc_off[2], bytes;
 };
 
+// What a call's page tables decide of its plan.
+enum : unsigned { kPlanRepeat = 1, kPlanLong = 2, kPlanChoices = 4 };
+
 // Row tile for entities of `rows` query rows: up to 64 the kernel for few rows
 // a key, in its narrowest shape that holds them; beyond, the tensor cores'.
 // 48 sequences of 4000 rows, 8 KV heads: 4 rows 101 us (in tiles of 32: 105), 32
-// rows 110 us (in tiles of 64: 168).  33 to 64 rows lie between: 48 sequences
-// of 16 tokens on 200 rows take 29 us (the other kernel's starts and ends: 33),
-// on 2000 rows 102 us (91).
-int tile_rows(int64_t rows) {
-  return rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : mllb::AttnMany<128>::kRows;
+// rows 110 us (in tiles of 64: 168).  33 to 64 rows lie between, and the length
+// decides: 48 sequences of 16 tokens on 60 rows take the few-row kernel 19 us and
+// the other, whose items start and end dearer, 22; on 700 rows 53 and 48, on 4000
+// rows 172 and 133.
+int tile_rows(int64_t rows, bool longs) {
+  return rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 && !longs ? 64 : mllb::AttnMany<128>::kRows;
+}
+
+// Whether prefix and own rows run as one softmax a sequence (paged_plan).
+bool one_softmax(int64_t seq_rows, int64_t seqs, int64_t groups, bool repeat) {
+  return groups == 0 || groups >= seqs || seq_rows >= 64 || repeat;
 }
 
 // Whether every sequence reads its group's prefix for itself although few rows
 // each do so: the prefixes come from L2 after the first time, and one pass has
 // less to join and to launch.  By the bytes read again at most, as the tables'
 // widths bound them: 64 MB against a pass of prefixes and own rows (fp16, heads
-// of 128, own rows 100; 16 sequences of a 1000-row prefix, 60 MB, 18.5 us
-// against 19.4; of 4000, 236 MB, 32.8 against 24.5), 192 MB against a pass each
-// (40 of 1000, 156 MB, 28.3 against 36.9; of 4000, 614 MB, 63 against 41.6).
-bool prefix_repeats(const mllb_paged_attn* p, const mllb_paged_cache* c) {
-  const int64_t again = (p->seqs - p->groups) * p->prefix_width * c->page_size * c->kv_heads * c->head_dim * 4;
-  const bool together = p->groups && (p->tokens * (p->q_heads / c->kv_heads) + p->groups - 1) / p->groups <= 64;
-  return p->groups && again <= (together ? 64ll : 192ll) << 20;
+// of 128, own rows 100; 16 sequences of a 1000-row prefix, 60 MB, 18.1 us
+// against 19.5; of 4000, 236 MB, 32.4 against 22.7), 192 MB against a pass each
+// (40 of 1000, 156 MB, 28.0 against 31.8; of 4000, 614 MB, 63 against 37).
+// And whether a sequence's item is long by the same bound: 512 rows and more
+// (tile_rows).
+unsigned plan_choice(const mllb_paged_attn* p, const mllb_paged_cache* c) {
+  const int64_t prefix = p->groups ? p->prefix_width * c->page_size : 0, rows = p->tokens * (p->q_heads / c->kv_heads);
+  const int64_t again = (p->seqs - p->groups) * prefix * c->kv_heads * c->head_dim * 4;
+  const bool together = p->groups && (rows + p->groups - 1) / p->groups <= 64;
+  const bool repeat = p->groups && again <= (together ? 64ll : 192ll) << 20;
+  const int64_t keys = p->table_width * c->page_size +
+                       (one_softmax((rows + p->seqs - 1) / p->seqs, p->seqs, p->groups, repeat) ? prefix : 0);
+  return (repeat ? kPlanRepeat : 0u) | (keys >= 512 ? kPlanLong : 0u);
 }
 
 // Mean query rows (tokens x query heads of a KV head) of a sequence and of a
 // group decide the shape.  A sequence with a row tile's worth of rows shares
 // nothing more by going through its group, so prefix and own rows then run as
-// one softmax (no segments to join); so they do where `repeat` says.  Otherwise
-// the prefix runs once a group (16 sequences over a prefix of 8000 rows: 32 rows
-// each 55 us, as one softmax 142; 128 rows each 109 us, as one softmax 112): in
-// one pass with the own rows where a group's rows fit one tile, in a pass of its
-// own on the tensor cores beyond.
+// one softmax (no segments to join); so they do where kPlanRepeat says.  Otherwise
+// the prefix runs once a group (16 sequences over a prefix of 8000 rows: up to 32
+// rows each 49 us, as one softmax 84; up to 128 rows each 98 and 103): in one
+// pass with the own rows where a group's rows fit one tile, in a pass of its own
+// on the tensor cores beyond.
 int paged_plan(int64_t tokens, int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t seqs, int64_t groups,
-               bool repeat, int dev, PagedPlan* p) {
+               unsigned choice, int dev, PagedPlan* p) {
+  const bool repeat = choice & kPlanRepeat, longs = choice & kPlanLong;
   const int64_t ratio = q_heads / kv_heads;
   const int64_t seq_rows = (tokens * ratio + seqs - 1) / seqs;
   const int64_t group_rows = groups ? (tokens * ratio + groups - 1) / groups : 0;
   memset(p, 0, sizeof(*p));
   p->passes = 1;
-  if (groups == 0 || groups >= seqs || seq_rows >= 64 || repeat) {
+  if (one_softmax(seq_rows, seqs, groups, repeat)) {
     p->mode[0] = groups ? mllb::kAttnConcat : mllb::kAttnOwn;
-    p->rows[0] = tile_rows(seq_rows);
+    p->rows[0] = tile_rows(seq_rows, longs);
     p->entities[0] = static_cast<int>(seqs);
   } else if (group_rows <= 64) {
     p->mode[0] = mllb::kAttnBoth;
-    p->rows[0] = tile_rows(group_rows);
+    p->rows[0] = tile_rows(group_rows, false);
     p->entities[0] = static_cast<int>(groups + seqs);
     p->dense[0] = 1;
   } else {
     p->passes = 2;
     p->mode[0] = mllb::kAttnPrefix;
-    p->rows[0] = tile_rows(group_rows);
+    p->rows[0] = tile_rows(group_rows, false);
     p->entities[0] = static_cast<int>(groups);
     p->mode[1] = mllb::kAttnOwn;
-    p->rows[1] = tile_rows(seq_rows);
+    p->rows[1] = tile_rows(seq_rows, longs);
     p->entities[1] = static_cast<int>(seqs);
     p->dense[0] = p->dense[1] = 1;
   }
@@ -283,7 +299,8 @@ int launch_attn(const mllb::AttnArgs& a, const mllb::AttnPass& pass, const CUten
 // Warps that join one row: four while all rows' fit on the SMs at once (few rows
 // of long contexts have tens of segments each; one sequence of 4096 rows 12.4 us,
 // with one warp a row 17.5), otherwise one, which has less to gather (16
-// sequences of up to 8 tokens over a prefix of 8000 rows 55 us, with four 68).
+// sequences of up to 8 tokens over a prefix of 8000 rows 55 us, with four 68,
+// both before the tensor cores' kernel stored whole lines).
 int join_parts(const mllb::AttnArgs& a, int dev) {
   return static_cast<int64_t>(a.tokens) * a.kv_heads * a.ratio * 4 <= 32ll * sm_count(dev) ? 4 : 1;
 }
@@ -383,10 +400,13 @@ int64_t mllb_paged_attention_workspace(int64_t tokens, int64_t q_heads, int64_t 
   int dev, rc;
   if ((rc = check_attn_sizes(tokens, q_heads, kv_heads, head_dim, seqs, groups))) return rc;
   if ((rc = current_device(&dev))) return rc;
-  PagedPlan plan, other;  // which of them a call takes depends on its page tables, too
-  if ((rc = paged_plan(tokens, q_heads, kv_heads, head_dim, seqs, groups, false, dev, &plan))) return rc;
-  if ((rc = paged_plan(tokens, q_heads, kv_heads, head_dim, seqs, groups, true, dev, &other))) return rc;
-  return plan.bytes > other.bytes ? plan.bytes : other.bytes;
+  int64_t most = 0;  // of the plans that the page tables decide between
+  for (unsigned choice = 0; choice < kPlanChoices; ++choice) {
+    PagedPlan plan;
+    if ((rc = paged_plan(tokens, q_heads, kv_heads, head_dim, seqs, groups, choice, dev, &plan))) return rc;
+    if (plan.bytes > most) most = plan.bytes;
+  }
+  return most;
 }
 
 int mllb_paged_attention(const mllb_paged_attn* p, const mllb_paged_cache* cache, void* workspace, int64_t workspace_bytes,
@@ -413,8 +433,8 @@ int mllb_paged_attention(const mllb_paged_attn* p, const mllb_paged_cache* cache
   int dev;
   if ((rc = current_device(&dev))) return rc;
   PagedPlan plan;
-  const bool repeat = prefix_repeats(p, cache);
-  if ((rc = paged_plan(p->tokens, p->q_heads, cache->kv_heads, cache->head_dim, p->seqs, p->groups, repeat, dev, &plan)))
+  const unsigned choice = plan_choice(p, cache);
+  if ((rc = paged_plan(p->tokens, p->q_heads, cache->kv_heads, cache->head_dim, p->seqs, p->groups, choice, dev, &plan)))
     return rc;
   if (workspace_bytes < plan.bytes)
     return fail(MLLB_EINVAL, "workspace of %lld bytes, %lld needed", static_cast<long long>(workspace_bytes),
