@@ -173,7 +173,7 @@ __device__ __forceinline__ void beam_best(BeamScratch& sh, int total, int n, uns
 // candidate.  Bound: issue slots, about 8 a logit (unpack, NaN, maximum,
 // difference, product, ex2, sum), rather than its 2 or 4 bytes from HBM, and
 // for short chunks the latencies of the selection.  Both kernels, 32 x 8 rows of
-// 151936 in bf16: n = 8 33 us, n = 16 with a quarter of the beams done 39; the
+// 151936 in bf16: n = 8 33 us, n = 16 with some of the beams done 39; the
 // bytes alone 12.  4 rows in fp32: 11.
 template <int kType, bool kVector>
 __global__ void __launch_bounds__(kBeamThreads, 4) beam_scan_kernel(const BeamArgs a) {
