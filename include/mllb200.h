@@ -553,7 +553,8 @@ typedef struct mllb_paged_cache {
  *   rows[t] of sequence seq[t] (seq NULL: of sequence t).
  * A negative rows[t] is padding: nothing is stored for it, q_out neither.  A
  * row without a page stores q_out only (and sets bit 8).  No (sequence, row)
- * may come twice in a call.  fp32 arithmetic, fp64 angles.
+ * may come twice in a call, and q_out must not overlap qkv.  fp32 arithmetic,
+ * fp64 angles.
  */
 typedef struct mllb_paged_append {
     const void *qkv;
@@ -581,9 +582,9 @@ int mllb_paged_qkv_append(const mllb_paged_append *args, const mllb_paged_cache 
  * nothing gets zeros; tokens behind q_start[seqs] stay as they are.  Rows
  * behind a sequence's length may hold anything, NaN too; the visible ones,
  * and those of a sequence's later tokens, must be finite.  q head h reads KV
- * head h / (q_heads / kv_heads).  q and out have the cache's type; fp32
- * softmax and sums, the weights rounded to the cache's type for the products
- * with V.  workspace: mllb_paged_attention_workspace bytes (the number
+ * head h / (q_heads / kv_heads).  q and out have the cache's type, and out
+ * may be q itself; fp32 softmax and sums, the weights rounded to the cache's
+ * type for the products with V.  workspace: mllb_paged_attention_workspace bytes (the number
  * depends on the current device), 16-byte aligned, any contents; calls that
  * share it must not overlap on the GPU.  seqs + groups <= 2048.
  */

@@ -222,7 +222,8 @@ int check_attn_sizes(int64_t tokens, int64_t q_heads, int64_t kv_heads, int64_t 
   if (head_dim != 64 && head_dim != 128)
     return fail(MLLB_EUNSUPPORTED, "head_dim=%lld is not 64 or 128", static_cast<long long>(head_dim));
   if (q_heads % kv_heads) return fail(MLLB_EINVAL, "q_heads is not a multiple of kv_heads");
-  if (q_heads > 1024 || tokens > (1 << 24)) return fail(MLLB_EINVAL, "q_heads or tokens out of range");
+  if (q_heads > 1024 || tokens > (1 << 24) || tokens * q_heads >= (1ll << 31))
+    return fail(MLLB_EINVAL, "q_heads or tokens out of range");
   if (groups > seqs) return fail(MLLB_EINVAL, "more groups than sequences");
   if (seqs + groups > mllb::kAttnMaxEntities)
     return fail(MLLB_EUNSUPPORTED, "more than %d sequences and groups", mllb::kAttnMaxEntities);
@@ -353,6 +354,9 @@ int mllb_paged_qkv_append(const mllb_paged_append* p, const mllb_paged_cache* ca
       (p->k_gamma && !aligned(p->k_gamma, 4)))
     return fail(MLLB_EALIGN, "q_out and freqs need 8-byte, the other pointers 4-byte alignment");
   if (!(p->eps >= 0.0)) return fail(MLLB_EINVAL, "eps must not be negative");
+  const auto in = reinterpret_cast<uintptr_t>(p->qkv), to = reinterpret_cast<uintptr_t>(p->q_out);
+  if (to < in + ((p->tokens - 1) * p->qkv_stride + heads * d) * size && in < to + p->tokens * p->q_heads * d * 2)
+    return fail(MLLB_EINVAL, "q_out must not overlap qkv");
   a.qkv = p->qkv;
   a.positions = p->positions;
   a.rows = p->rows;
@@ -428,6 +432,8 @@ int mllb_paged_attention(const mllb_paged_attn* p, const mllb_paged_cache* cache
   const int64_t strides[4] = {p->q_token_stride, p->q_head_stride, p->out_token_stride, p->out_head_stride};
   for (int64_t s : strides)
     if (s < 0 || s % 8) return fail(MLLB_EALIGN, "q and out strides must be multiples of 8 elements (16 bytes)");
+  if ((p->tokens > 1 && p->out_token_stride < cache->head_dim) || (p->q_heads > 1 && p->out_head_stride < cache->head_dim))
+    return fail(MLLB_EINVAL, "rows of out overlap");
   if (!aligned(p->q, 16) || !aligned(p->out, 16) || !aligned(workspace, 16))
     return fail(MLLB_EALIGN, "q, out and workspace must be 16-byte aligned");
   int dev;

@@ -778,7 +778,9 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     q_start[b + 1] - 1 (None: one each), the last ones of those rows, each seeing the rows up to its own.  Sequences
     group_start[g] .. group_start[g + 1] - 1 (None: all) see the prefix_lens[g] rows of prefix_table[g] too; these are
     read once for all of a group's sequences.  A token that sees nothing gets zeros; tokens behind q_start[-1] are left
-    as they are.  scale: 1 / sqrt(head_dim) unless given."""
+    as they are.  What a row's mask hides may hold anything behind a sequence's length; rows that later tokens of the
+    sequence see must be finite.  At most 2048 sequences and groups.  scale: 1 / sqrt(head_dim) unless given.  out may
+    be q."""
     return native().paged_attention(q, k_cache, v_cache, page_table, seq_lens, prefix_table, prefix_lens, group_start,
                                     q_start, scale, out, workspace, pdl)
 
@@ -791,7 +793,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, n: int | None = None
 
     logits [batch, beams, vocab] in fp32, fp16 or bf16, scores fp32 [batch, beams].  -inf logits are never chosen; a
     beam that is done (bool or uint8 [batch, beams]) offers only end_token at its score.  Places without a candidate
-    hold -inf, -1, -1.  out: the three result tensors, to write into."""
+    hold -inf, -1, -1.  out: the three result tensors, to write into (the first may be scores where n is beams)."""
     return native().beam_select(logits, scores, n, done, end_token, out, workspace, pdl)
 
 

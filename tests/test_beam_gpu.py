@@ -156,3 +156,15 @@ def test_select_captured_and_on_another_stream():
     side.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(side):
         check(logits, scores, 6)
+
+
+def test_select_into_its_scores_and_shared_logits():
+    """New scores written over the old ones; logits that all beams share (stride 0)."""
+    logits, scores = random(3, 5, 7000, torch.float32, 21)
+    dev, sc = logits[:, :1].cuda().expand(3, 5, 7000), scores.cuda()
+    want = P.select(logits[:, :1].expand(3, 5, 7000).contiguous(), scores, 5, None, -1)
+    out = (sc, torch.empty(3, 5, dtype=torch.int32, device="cuda"), torch.empty(3, 5, dtype=torch.int32, device="cuda"))
+    alone = ops.beam_select(dev, sc)
+    ops.beam_select(dev, sc, out=out)
+    assert torch.equal(out[1].cpu(), want[1]) and torch.equal(out[2].cpu(), want[2])
+    assert all(torch.equal(x, y) for x, y in zip(out, alone))

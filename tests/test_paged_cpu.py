@@ -150,7 +150,8 @@ def test_bad_caches(kw, code):
     (dict(tokens=3), _lib.MLLB_EINVAL), (dict(rot_dim=0), _lib.MLLB_EINVAL), (dict(rot_dim=127), _lib.MLLB_EINVAL),
     (dict(rot_dim=130), _lib.MLLB_EINVAL), (dict(qkv_stride=1000), _lib.MLLB_EINVAL), (dict(qkv_stride=1026), _lib.MLLB_EALIGN),
     (dict(qkv=4104), _lib.MLLB_EALIGN), (dict(qkv_type=3), _lib.MLLB_EINVAL), (dict(eps=-1.0), _lib.MLLB_EINVAL),
-    (dict(eps=math.nan), _lib.MLLB_EINVAL), (dict(q_heads=0), _lib.MLLB_EINVAL)])
+    (dict(eps=math.nan), _lib.MLLB_EINVAL), (dict(q_heads=0), _lib.MLLB_EINVAL),
+    (dict(q_out=4096 + 1024 * 4 + 1024 * 4 - 8), _lib.MLLB_EINVAL)])  # q_out over the end of qkv
 def test_bad_appends(kw, code):
     assert _lib.lib().mllb_paged_qkv_append(c_append(**kw), c_cache(), 0, None) == code
 
@@ -162,7 +163,8 @@ def test_more_entries_refuse():
     for kw, code in [(dict(q=None), _lib.MLLB_EINVAL), (dict(tokens=3), _lib.MLLB_EINVAL), (dict(q_heads=3), _lib.MLLB_EINVAL),
                      (dict(groups=1), _lib.MLLB_EINVAL), (dict(groups=3, prefix_table=4096, prefix_lens=4096), _lib.MLLB_EINVAL),
                      (dict(groups=2, prefix_table=4096, prefix_lens=4096, prefix_width=2), _lib.MLLB_EINVAL),
-                     (dict(q_head_stride=130), _lib.MLLB_EALIGN), (dict(out=4104), _lib.MLLB_EALIGN),
+                     (dict(q_head_stride=130), _lib.MLLB_EALIGN), (dict(out_token_stride=0), _lib.MLLB_EINVAL),
+                     (dict(out_head_stride=0), _lib.MLLB_EINVAL), (dict(out_head_stride=64), _lib.MLLB_EINVAL), (dict(out=4104), _lib.MLLB_EALIGN),
                      (dict(scale=math.inf), _lib.MLLB_EINVAL), (dict(scale=math.nan), _lib.MLLB_EINVAL),
                      (dict(table_width=0), _lib.MLLB_EINVAL), (dict(table_width=1 << 27), _lib.MLLB_EINVAL),
                      (dict(tokens=3000, seqs=3000), _lib.MLLB_EUNSUPPORTED)]:

@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import paged_util as P
-from mojo_llm_lab_b200 import ops
+from mojo_llm_lab_b200 import _lib, ops
 
 pytestmark = pytest.mark.gpu
 
@@ -387,6 +387,37 @@ def test_captured_attention_follows_lengths(prefix, apart):
         check_attention(c, out)
 
 
+@pytest.mark.parametrize("lens,news,prefix", [
+    ([700, 90, 1], None, []), ([300, 170], [200, 170], [100]), ([64] * 9, None, [500]), ([30] * 70, None, [300])])
+def test_attention_into_its_queries(lens, news, prefix):
+    c = attention_case(lens, news, prefix, seed=17)
+    want = run_attention(c)
+    q = c["q"].cuda()
+    assert run_attention(c, q=q, out=q) is q
+    assert torch.equal(q, want)
+
+
+@pytest.mark.parametrize("news", [3, 200])
+def test_attention_of_one_query_for_all_tokens(news):
+    """q with stride 0 over the tokens."""
+    c = attention_case([300], [news], seed=18)
+    one = c["q"][:1].cuda()
+    out = run_attention(c, q=one.expand(news, -1, -1))
+    c["q"] = c["q"][:1].expand(news, -1, -1).contiguous()
+    check_attention(c, out)
+
+
+def test_attention_most_sequences():
+    """2047 sequences and their one prefix, as one softmax and apart; one more is refused."""
+    lens = [i % 19 for i in range(2047)]
+    for apart in (False, True):
+        c = attention_case(lens, prefix=[33], hq=2, hk=1, d=64, seed=19, apart=apart)
+        check_attention(c, run_attention(c))
+    c = attention_case(lens + [3], prefix=[33], hq=2, hk=1, d=64, seed=19, apart=False)
+    with pytest.raises(_lib.MllbError, match="2048"):
+        run_attention(c)
+
+
 # ------------------------------------------------------------------ reorder
 
 @pytest.mark.parametrize("batch,beams,layers,heads,page,d,dtype,rows_first", [
@@ -491,3 +522,46 @@ def test_beam_decoding_steps():
         held = set(table.flatten().tolist())
         free = sorted((set(free) | {int(f) for f in fresh} | set(range(used_pages, pages))) - held - {-1})
         tokens = picked.cpu().view(-1).long()
+
+
+def test_captured_step_of_all_operators():
+    """Append, attention, selection and reordering in one graph, replayed on other states: as the calls one by one."""
+    batch, beams, hq, hk, d, page, vocab, r = 2, 3, 4, 2, 64, 16, 300, 6
+    freqs, _ = ops.rope_frequencies(d)
+    g = torch.Generator().manual_seed(9)
+    shapes = dict(qkv=(r, (hq + 2 * hk) * d), head=(hq * d, vocab))
+    fixed = {k: torch.randn(*v, generator=g).cuda() for k, v in shapes.items()}
+    kc, vc = (torch.randn(40, hk, page, d, generator=g).to(F16).cuda() for _ in range(2))
+    i32 = dict(dtype=torch.int32, device="cuda")
+    table, fresh = torch.arange(12, **i32).view(r, 2), torch.arange(20, 20 + r, **i32)
+    prefix, plens, starts = torch.arange(30, 34, **i32).view(2, 2), torch.tensor([20, 32], **i32), torch.tensor([0, 3, 6], **i32)
+    state = dict(rows=torch.zeros(r, **i32), lens=torch.ones(r, **i32), positions=torch.zeros(r, **i32),
+                 scores=torch.zeros(batch, beams, device="cuda"), kc=kc, vc=vc)
+
+    def step(s):
+        q = ops.paged_qkv_append(fixed["qkv"], s["positions"], s["rows"], table, s["kc"], s["vc"], hq, freqs)
+        out = ops.paged_attention(q, s["kc"], s["vc"], table, s["lens"], prefix, plens, starts)
+        logits = (out.view(r, -1, 1).float() * fixed["head"]).sum(1).view(batch, beams, vocab)
+        scores, tokens, parents = ops.beam_select(logits, s["scores"])
+        return (q, out, scores, tokens, parents, *ops.beam_reorder(parents, table, s["lens"], fresh, s["kc"], s["vc"]))
+
+    step({k: v.clone() for k, v in state.items()})
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(state)
+    for at in (0, 5, 16, 30):
+        state["rows"].fill_(at)
+        state["lens"].fill_(at + 1)
+        state["positions"].fill_(at + 20)
+        state["scores"].copy_(torch.randn(batch, beams, generator=g))
+        state["kc"].normal_()
+        state["vc"].normal_()
+        copy = {k: v.clone() for k, v in state.items()}
+        graph.replay()
+        want = step(copy)
+        torch.cuda.synchronize()
+        for x, y in zip(got, want):
+            assert torch.equal(x, y)
+        assert torch.equal(state["kc"], copy["kc"]) and torch.equal(state["vc"], copy["vc"])
+    assert ops.device_error() == 0
