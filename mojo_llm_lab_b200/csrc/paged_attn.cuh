@@ -150,8 +150,16 @@ __device__ __forceinline__ int attn_key_tiles(const AttnEntity& n, int ratio, in
   return max((n.plen + KT - 1) / KT + (attn_limit(n, last / ratio) + KT - 1) / KT, least);
 }
 
-// First pair of CTA c's share.  No more CTAs take part than there are pairs,
-// so every one of an item's CTAs, first to last, has a segment of it.
+// An item's length on the line: its key tiles, and what its start and end cost
+// beside them, on the tensor cores about as long as two key tiles (queries, first
+// scores, results).  Without that the CTAs of short items end last: one prompt of
+// 8000 tokens, whose first row tiles see one key tile, 638 -> 451 us (counted as
+// one tile 515, as three 454), of 1000 tokens 41 -> 32.
+__host__ __device__ constexpr int attn_ends(int R) { return R > 64 ? 2 : 0; }
+__device__ __forceinline__ int attn_cost(int key_tiles, int R) { return key_tiles > 0 ? key_tiles + attn_ends(R) : 0; }
+
+// First place of CTA c's share.  No more CTAs take part than there are places,
+// so every one of an item's CTAs, first to last with a key tile, has a segment.
 __device__ __forceinline__ int attn_share(int total, int ctas, int c) {
   return static_cast<int>(static_cast<long long>(total) * c / ctas);
 }
@@ -161,11 +169,11 @@ struct AttnCursor {
   int total;       // all pairs
   int left;        // key tiles left in the share
   int e, t, h;     // entity, row tile, KV head
-  int begin;       // first key tile of the segment
+  int begin;       // where the share starts in the item
   int item;        // number of the item on the line
 };
 
-// Entity e's (row tile, KV head, key tile) pairs and its items; 0 past the last.
+// Entity e's length on the line (attn_cost of its items) and its items; 0 past the last.
 template <int R, int KT>
 __device__ __forceinline__ void attn_work(const AttnArgs& a, const AttnPass& pass, int e, int* pairs, int* items) {
   int w = 0, t = 0;
@@ -173,9 +181,9 @@ __device__ __forceinline__ void attn_work(const AttnArgs& a, const AttnPass& pas
     const AttnEntity ent = attn_entity(a, pass.mode, e);
     t = attn_row_tiles(ent, a.ratio, R);
     if (ent.causal && ent.ntok > 1) {
-      for (int i = 0; i < t; ++i) w += attn_key_tiles(ent, a.ratio, i, R, KT, !pass.dense);
+      for (int i = 0; i < t; ++i) w += attn_cost(attn_key_tiles(ent, a.ratio, i, R, KT, !pass.dense), R);
     } else if (t > 0) {
-      w = t * attn_key_tiles(ent, a.ratio, 0, R, KT, !pass.dense);
+      w = t * attn_cost(attn_key_tiles(ent, a.ratio, 0, R, KT, !pass.dense), R);
     }
   }
   *pairs = w * a.kv_heads;
@@ -193,11 +201,11 @@ __device__ __forceinline__ AttnCursor attn_locate(const AttnArgs& a, const AttnP
   c.left = attn_share(total, ctas, cta + 1) - attn_share(total, ctas, cta);
   c.e = e;
   const AttnEntity ent = attn_entity(a, pass.mode, e);
-  int k = attn_key_tiles(ent, a.ratio, 0, R, KT, !pass.dense);
+  int k = attn_cost(attn_key_tiles(ent, a.ratio, 0, R, KT, !pass.dense), R);
   if (ent.causal && ent.ntok > 1) {
     while (rest >= a.kv_heads * k) {
       rest -= a.kv_heads * k;
-      k = attn_key_tiles(ent, a.ratio, ++c.t, R, KT, !pass.dense);
+      k = attn_cost(attn_key_tiles(ent, a.ratio, ++c.t, R, KT, !pass.dense), R);
     }
   } else {
     c.t = rest / (a.kv_heads * k);
@@ -303,33 +311,41 @@ struct AttnWalk {
     if (c.left > 0) ent = attn_entity(a, mode, c.e);
   }
   __device__ bool next(AttnSegment* s) {
-    if (c.left <= 0) return false;
-    int k = 0;
-    for (;;) {  // skip row tiles that see nothing and entities without rows
-      const int tiles = attn_row_tiles(ent, a.ratio, R);
-      if (c.t < tiles) {
-        k = attn_key_tiles(ent, a.ratio, c.t, R, KT, least);
-        if (k > 0) break;
-        ++c.t;
-        c.item += a.kv_heads;
-      } else {
-        if (++c.e >= entities) return false;
-        c.t = 0;
-        ent = attn_entity(a, mode, c.e);
+    while (c.left > 0) {
+      int k = 0;
+      for (;;) {  // skip row tiles that see nothing and entities without rows
+        const int tiles = attn_row_tiles(ent, a.ratio, R);
+        if (c.t < tiles) {
+          k = attn_key_tiles(ent, a.ratio, c.t, R, KT, least);
+          if (k > 0) break;
+          ++c.t;
+          c.item += a.kv_heads;
+        } else {
+          if (++c.e >= entities) return false;
+          c.t = 0;
+          ent = attn_entity(a, mode, c.e);
+        }
       }
+      // The key tiles stand behind the item's start on the line; a share that
+      // ends before them leaves the item to the next CTA.
+      const int end = min(attn_cost(k, R), c.begin + c.left);
+      const int first = max(c.begin - attn_ends(R), 0), past = max(end - attn_ends(R), 0);
+      const int t = c.t, h = c.h, item = c.item;
+      c.left -= end - c.begin;
+      c.begin = 0;
+      ++c.item;
+      if (++c.h == a.kv_heads) c.h = 0, ++c.t;
+      if (first >= past) continue;
+      s->ent = ent;
+      s->t = t;
+      s->h = h;
+      s->begin = first;
+      s->end = past;
+      s->of = k;
+      s->item = item;
+      return true;
     }
-    s->ent = ent;
-    s->t = c.t;
-    s->h = c.h;
-    s->begin = c.begin;
-    s->end = min(k, c.begin + c.left);
-    s->of = k;
-    s->item = c.item;
-    c.left -= s->end - s->begin;
-    c.begin = 0;
-    ++c.item;
-    if (++c.h == a.kv_heads) c.h = 0, ++c.t;
-    return true;
+    return false;
   }
 };
 

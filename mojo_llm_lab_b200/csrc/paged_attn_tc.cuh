@@ -32,7 +32,7 @@
 // exponentials as many (16 a cycle), the rest of the softmax issue slots beside
 // them; the two streams hide less of one behind the other than they might, and
 // the clock falls under this load.  Prompts of 1 to 1024 tokens behind a prefix of 1500 rows
-// (119 GFLOP) take 133 us, 0.90 PFLOP/s, and one of 8000 tokens 632 us, 0.83.
+// (119 GFLOP) take 131 us, 0.91 PFLOP/s, and one of 8000 tokens 451 us, 1.16.
 #pragma once
 
 #include "paged_attn.cuh"

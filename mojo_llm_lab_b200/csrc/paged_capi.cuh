@@ -475,7 +475,7 @@ int mllb_paged_attention(const mllb_paged_attn* p, const mllb_paged_cache* cache
   for (int i = 0; i < plan.passes; ++i) {
     // The line of (item, key tile) pairs is counted in 32 bits.
     const int64_t items = cache->kv_heads * ((p->tokens * a.ratio + plan.rows[i] - 1) / plan.rows[i] + plan.entities[i]);
-    const int64_t most = ((p->table_width + (p->groups ? p->prefix_width : 0)) * cache->page_size) / plan.keys[i] + 2;
+    const int64_t most = ((p->table_width + (p->groups ? p->prefix_width : 0)) * cache->page_size) / plan.keys[i] + 2 + mllb::attn_ends(plan.rows[i]);
     if (items * most >= (1ll << 31)) return fail(MLLB_EUNSUPPORTED, "too many rows x keys for one call");
     pass[i].mode = plan.mode[i];
     pass[i].entities = plan.entities[i];

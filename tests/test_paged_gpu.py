@@ -228,7 +228,9 @@ def test_attention_shared_prefixes(seqs, prefix, group_start, hq, hk, dtype, apa
     ([200, 150, 90], [64, 2, 90], [500], 8, 2, 128), ([600, 550], [600, 400], [333], 8, 2, 128),
     ([64, 64, 64, 64], [4, 4, 3, 2], [1000], 8, 2, 128),
     ([100, 90, 60], [12, 9, 11], [], 8, 2, 128), ([600, 511, 30], [12, 9, 11], [], 8, 2, 64),  # short, long tables
-    ([600, 511, 30], [12, 9, 11], [70], 8, 2, 128), ([1100], [1030], [129], 2, 1, 64)])
+    ([600, 511, 30], [12, 9, 11], [70], 8, 2, 128),
+    (list(range(70, 110)), list(range(70, 110)), [], 8, 2, 64),  # items of one or two tiles: shares start anywhere in them
+    ([130] * 30, [100 + i % 7 for i in range(30)], [65], 4, 1, 128), ([1500], [1500], [], 4, 2, 64), ([1100], [1030], [129], 2, 1, 64)])
 @pytest.mark.parametrize("dtype,apart", [(F16, True), (BF16, True), (F16, False)])
 def test_attention_many_tokens(lens, news, prefix, hq, hk, d, dtype, apart):
     c = attention_case(lens, news, prefix, hq=hq, hk=hk, d=d, dtype=dtype, seed=sum(lens), apart=apart)
