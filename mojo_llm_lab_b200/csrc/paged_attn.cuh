@@ -443,6 +443,14 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+// Weights of a row are 2^(x - maximum + lift).  fp16 rounds to zero what is
+// below 2^-25, so without a lift a long tail 17.5 nats below one key vanished
+// from the products while the sum counted it (4000 such keys: 1e-4 of the
+// result).  2^15 is fp16's largest power of two.  Sums and accumulators carry
+// the same factor, which the division takes out; a segment's statistics are
+// (maximum - lift, sum).  bf16 has fp32's exponents and needs none.
+__host__ __device__ constexpr float attn_lift(bool bf16, int most) { return bf16 ? 0.0f : static_cast<float>(most); }
+
 // ------------------------------------------------------------ few rows a key
 //
 // Row tiles of R = 16, 32 or 64: a key is used for at most R rows, so HBM
@@ -477,6 +485,7 @@ __global__ void __launch_bounds__(160, 2)
                           const __grid_constant__ CUtensorMap vmap) {
   using C = AttnFew<D, R>;
   constexpr int KT = C::kKeys;
+  constexpr float kLift = attn_lift(kBf16, 15);
   extern __shared__ __align__(1024) uint8_t attn_smem[];
   uint8_t* ring = attn_smem;
   float* join = reinterpret_cast<float*>(attn_smem + C::kStages * C::kStage);
@@ -619,8 +628,8 @@ __global__ void __launch_bounds__(160, 2)
         m0 = fmaxf(m0, __shfl_xor_sync(0xffffffffu, m0, d));
         m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, d));
       }
-      const float z0 = m0 == -INFINITY ? 0.0f : m0, z1 = m1 == -INFINITY ? 0.0f : m1;
-      const float f0 = ex2(top[0] - z0), f1 = ex2(top[1] - z1);
+      const float f0 = ex2(top[0] - (m0 == -INFINITY ? 0.0f : m0)), f1 = ex2(top[1] - (m1 == -INFINITY ? 0.0f : m1));
+      const float z0 = m0 == -INFINITY ? 0.0f : m0 - kLift, z1 = m1 == -INFINITY ? 0.0f : m1 - kLift;
       top[0] = m0;
       top[1] = m1;
       sum[0] *= f0;
@@ -641,9 +650,10 @@ __global__ void __launch_bounds__(160, 2)
         sum[0] += x[i][0] + x[i][1];
         sum[1] += x[i][2] + x[i][3];
       }
-      // P in the cache's type (a factor 1 + 2^-11 or 2^-8 at most on each
-      // weight; the sums keep the unrounded ones).  V rows behind the end of
-      // a sequence are anything at all, NaN too: those registers become zero.
+      // P in the cache's type: off by half a step, a factor 1 +- 2^-11 or 2^-8 at
+      // most, in fp16 from 2^-29 of the largest weight on and 2^-40 of that one
+      // below (attn_lift); the sums keep the unrounded weights.  V rows behind the
+      // end of a sequence are anything at all, NaN too: those registers become zero.
       const int held = tile.rows - tile.row0;
 #pragma unroll
       for (int i = 0; i < NT; i += 2) {
@@ -743,7 +753,7 @@ __global__ void __launch_bounds__(160, 2)
           for (int i = 0; i < 2; ++i) {
             if (token[i] < 0) continue;
             const long long r = static_cast<long long>(slot) * R + rw * 16 + g + i * 8;
-            if (tq == 0) pass.stats[r] = make_float2(top[i], sum[i]);
+            if (tq == 0) pass.stats[r] = make_float2(top[i] - kLift, sum[i]);
             float2* dst = reinterpret_cast<float2*>(pass.acc + r * D);
 #pragma unroll
             for (int c = 0; c < D / 8; ++c) dst[c * 4 + tq] = make_float2(acc[c][2 * i], acc[c][2 * i + 1]);

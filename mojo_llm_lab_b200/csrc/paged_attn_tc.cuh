@@ -18,9 +18,10 @@
 // is made.
 //
 // The running maximum is moved, and O rescaled, only when a row's scores
-// outgrow it by 2^8: until then its weights are up to 2^8 instead of up to 1,
-// which the 16-bit types hold as well and fp32 sums too.  After the first
-// tiles O is hardly ever touched by the softmax warps.
+// outgrow it by 2^8: until then its weights are up to 2^8 instead of up to 1
+// (2^15 with fp16's lift of 7), which the 16-bit types hold as well and fp32
+// sums too.  After the first tiles O is hardly ever touched by the softmax
+// warps.
 //
 // Where an item ends, the next one's queries and first keys are on their way
 // already: warp 10 posts segments two ahead and lets TMA bring their queries
@@ -154,6 +155,7 @@ __global__ void __launch_bounds__(384, 1)
                            const int q_by_tma) {
   using C = AttnMany<D>;
   constexpr int R = C::kRows, KT = C::kKeys, NS = C::kSlots;
+  constexpr float kLift = attn_lift(kBf16, 7);  // weights reach 2^8 above the running maximum's
   extern __shared__ __align__(1024) uint8_t attn_smem[];
   uint8_t* ring = attn_smem + C::kRingOff;
   uint64_t* full = reinterpret_cast<uint64_t*>(attn_smem + C::kBarOff);  // [NS] a tile has landed
@@ -489,9 +491,11 @@ __global__ void __launch_bounds__(384, 1)
             }
           }
         }
-        const float z = top == -INFINITY ? 0.0f : top;
+        const float z = top == -INFINITY ? 0.0f : top - kLift;
         float2 part[4] = {};
-        // P in the cache's type (half a step off at most; the sum keeps the unrounded weights).
+        // P in the cache's type: half a step off at most, in fp16 from 2^-21 of
+        // the running maximum's weight on, and 2^-32 of that one below; the sum
+        // keeps the unrounded weights.
 #pragma unroll
         for (int c = 0; c < KT; c += 32) {
           uint32_t p[16];
@@ -530,7 +534,7 @@ __global__ void __launch_bounds__(384, 1)
       if (!direct && !fits) record_error(kErrBadPage);
       const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
       const long long at = static_cast<long long>(slot) * R + stream * 128 + r;
-      if (keeps) pass.stats[at] = make_float2(top, sum);
+      if (keeps) pass.stats[at] = make_float2(top - kLift, sum);
       const int near = lane & ~7, piece = lane & 7;
       if (direct) {
         const long long place = mine.token * a.out_token + mine.head * a.out_head;

@@ -1,0 +1,55 @@
+"""Paged-cache operators at the edges: weights far below the largest, pages reserved ahead, nonsensical starts, memory."""
+import math
+
+import pytest
+import torch
+
+import paged_util as P
+from mojo_llm_lab_b200 import ops
+
+pytestmark = pytest.mark.gpu
+
+F16, BF16 = torch.float16, torch.bfloat16
+BAD_PAGE = 1 << 8
+
+
+@pytest.fixture(autouse=True)
+def no_device_error():
+    ops.device_error()
+    yield
+    torch.cuda.synchronize()
+    assert ops.device_error() == 0
+
+
+def ints(x):
+    return torch.tensor(x, dtype=torch.int32).cuda()
+
+
+# ------------------------------------------------------------------ weights far below the largest
+
+@pytest.mark.parametrize("hq,tokens", [(1, 1), (32, 1), (64, 1), (128, 1), (4, 64)])
+@pytest.mark.parametrize("at", [0, 1000, 3999])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_one_key_outweighs_a_long_tail(hq, tokens, at, dtype):
+    """One key 17.5 nats above 3999 others, whose values alone are not zero: each weighs less than half of fp16's
+    smallest number, all of them 1e-4.  300 sequences read the same pages, so that a CTA has whole items."""
+    n, page, d, seqs = 4000 + tokens - 1, 16, 64, 300
+    lines = -(-n // page)
+    kc, vc = torch.zeros(lines, 1, page, d, dtype=dtype), torch.ones(lines, 1, page, d, dtype=dtype)
+    kc[at // page, 0, at % page, 0] = 17.5
+    vc[at // page, 0, at % page] = 0.0
+    q = torch.zeros(seqs * tokens, hq, d, dtype=dtype)
+    q[..., 0] = 1.0
+    table = torch.arange(lines, dtype=torch.int32).repeat(seqs, 1).cuda()
+    more = dict(q_start=ints([tokens * i for i in range(seqs + 1)])) if tokens > 1 else {}
+    out = ops.paged_attention(q.cuda(), kc.cuda(), vc.cuda(), table, ints([n] * seqs), scale=1.0, **more)
+    seen = n - tokens + 1 + torch.arange(tokens, dtype=torch.float64).repeat(seqs)
+    tail = (seen - 1) * math.exp(-17.5)
+    want = (tail / (1 + tail))[:, None, None]
+    # Weights and result rounded once each; the scores' 25 powers of two and 2^x in fp32 (25.3 x 2^-23 + 2^-22); sums.
+    # fp16: a weight's steps are 2^-24 where the largest is 2^7 or more, so each is off by 2^-32 of the largest.
+    h = P.HALF[dtype]
+    bound = want * (2 * h + h * h + 26.3 * 2.0 ** -23 + (n / 8 + 64) * 2.0 ** -23)
+    if dtype == F16:
+        bound = bound + n * 2.0 ** -32 + 2.0 ** -25
+    assert ((out.double().cpu() - want).abs() <= bound).all()
