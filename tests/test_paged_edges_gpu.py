@@ -53,3 +53,28 @@ def test_one_key_outweighs_a_long_tail(hq, tokens, at, dtype):
     if dtype == F16:
         bound = bound + n * 2.0 ** -32 + 2.0 ** -25
     assert ((out.double().cpu() - want).abs() <= bound).all()
+
+
+# ------------------------------------------------------------------ sequences side by side
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_a_sequence_does_not_depend_on_its_neighbours_queries(dtype):
+    """The rows behind a sequence's last in its row tile are the next sequence's: they decide nothing.  The prefix's keys
+    grow, so that scores of large queries outgrow the running maximum again and again, those of small ones hardly."""
+    g = torch.Generator().manual_seed(3)
+    seqs, prefix, page, hq, hk, d = 40, 1500, 16, 32, 8, 128
+    news = [20, 100] * (seqs // 2)
+    table, pages, _ = P.tables(news + [prefix], page, 4)
+    kc, vc = P.cache(pages, hk, page, d, dtype, 4)
+    for i in range(prefix):
+        kc[int(table[seqs, i // page]), :, i % page] *= 0.1 + 0.9 * i / prefix
+    q = (torch.randn(sum(news), hq, d, generator=g) * 2).to(dtype).cuda()
+    short = torch.tensor([n == 20 for n in news]).repeat_interleave(torch.tensor(news)).cuda()
+    starts = ints([0] + torch.tensor(news).cumsum(0).tolist())
+    more = dict(prefix_table=table[seqs:].contiguous().cuda(), prefix_lens=ints([prefix]), q_start=starts)
+    own, kc, vc = table[:seqs, :-(-100 // page)].contiguous().cuda(), kc.cuda(), vc.cuda()
+    outs = []
+    for factor in (1.0, 4.0, 0.0):
+        other = torch.where(short[:, None, None], q, q * factor)
+        outs.append(ops.paged_attention(other, kc, vc, own, ints(news), **more)[short])
+    assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
