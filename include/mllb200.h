@@ -629,13 +629,15 @@ int mllb_beam_select(const mllb_beam_scores *args, float *out_scores, int32_t *o
                      void *workspace, int64_t workspace_bytes, unsigned flags, void *stream);
 
 /*
- * Row r = (entry, beam) of the page table and lengths becomes its parent's
- * (parents[r]: a beam of the same entry).  Whole pages are shared; the last,
+ * Row r = (entry, beam) of the page table, as far as its parent holds rows, and
+ * the length become the parent's (parents[r]: a beam of the same entry).  Columns
+ * behind stay the row's own (pages reserved ahead; no two rows may name one there),
+ * those where the row's own rows were become -1.  Whole pages are shared; the last,
  * part-full page goes on being written, so the first child of a parent (the
  * lowest r) keeps it and every other child gets fresh[r] in its place, with
  * the rows held copied for K and V of all layers; used[r] = 1 where fresh[r]
  * was taken.  fresh: distinct pages that no table line names.  A negative
- * parent ends the row (length 0, table -1), one past the beams also sets
+ * parent ends the row (length 0, table -1, reserved pages too), one past the beams also sets
  * device error bit 9 (mask 0x200).  table_out and lens_out must not overlap
  * the inputs.
  */

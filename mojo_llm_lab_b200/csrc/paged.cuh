@@ -256,8 +256,11 @@ struct ReorderArgs {
 constexpr int kReorderWarps = 8;
 constexpr int kReorderAhead = 8;
 
-// CTA (x, row): row's table and length come from its parent's row; the first
-// CTA writes them.  A page that is part full goes on being written by its
+// CTA (x, row): the pages of its rows and the length come from its parent's row;
+// the first CTA writes them.  Columns behind stay the row's own, pages that its
+// caller reserved ahead: the parent's would be every child's, who would write
+// over one another.  Where the row's own rows were is no such page (a sibling may
+// hold it), so those columns become -1.  A page that is part full goes on being written by its
 // beam, so only the first child of a parent keeps it: the others take
 // fresh[row], and the CTAs copy the rows held so far, one (layer, K or V,
 // head) a warp, 16 bytes a lane.  Bound: HBM where there is much to copy, as
@@ -292,8 +295,12 @@ __global__ void __launch_bounds__(kReorderWarps * 32) beam_reorder_kernel(const 
   const bool wants = valid && further && part > 0;
   const bool copies = wants && source >= 0 && source < a.cache.pages && target >= 0 && target < a.cache.pages;
   if (leads) {
+    const int32_t* mine = a.table + static_cast<long long>(row) * a.width;
+    const int held = len < 0 ? 0 : slot + (part > 0), len0 = a.lens[row];
+    const int past = len0 < 0 ? a.width : (len0 >> a.cache.page_shift) + ((len0 & ((1 << a.cache.page_shift) - 1)) > 0);
     for (int i = threadIdx.x; i < a.width; i += blockDim.x)
-      a.table_out[static_cast<long long>(row) * a.width + i] = copies && i == slot ? target : from[i];
+      a.table_out[static_cast<long long>(row) * a.width + i] =
+          i < held ? (copies && i == slot ? target : from[i]) : i < past ? -1 : mine[i];
     if (threadIdx.x == 0) {
       a.lens_out[row] = len;
       a.used[row] = copies;

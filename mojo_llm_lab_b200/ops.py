@@ -804,5 +804,6 @@ def beam_reorder(parents: torch.Tensor, page_table: torch.Tensor, seq_lens: torc
     them): (table, lens, used).  Beams go on writing their last page, so where several children share a part-full one,
     the first keeps it and each further row r gets the free page fresh[r] with the rows held so far copied (used[r] = 1)
     in the caches [pages, kv_heads, page_size, head_dim], or [layers, pages, ...] for all layers at once.  fresh pages
-    are distinct and not in the table.  A negative parent ends its row (length 0).  out: the three result tensors."""
+    are distinct and not in the table.  Columns behind the parent's rows stay the row's own (pages reserved ahead), or -1
+    where its own rows were.  A negative parent ends its row (length 0, table -1).  out: the three result tensors."""
     return native().beam_reorder(parents, page_table, seq_lens, fresh, k_cache, v_cache, out, pdl)

@@ -78,3 +78,56 @@ def test_a_sequence_does_not_depend_on_its_neighbours_queries(dtype):
         other = torch.where(short[:, None, None], q, q * factor)
         outs.append(ops.paged_attention(other, kc, vc, own, ints(news), **more)[short])
     assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
+
+
+# ------------------------------------------------------------------ pages reserved ahead
+
+def test_reorder_keeps_pages_reserved_ahead():
+    """Columns behind the parent's rows stay the row's own, unless the row's own rows were there."""
+    page, width = 16, 5
+    lens = [16, 33, 64, 0]
+    table = torch.arange(4 * width, dtype=torch.int32).view(4, width)
+    kc, vc = P.cache(30, 1, page, 64, F16, 3)
+    spare = torch.arange(20, 24, dtype=torch.int32)
+    #  children of a full page, of a part-full one twice, of a longer one, of an empty one
+    for parents in ([0, 0, 0, 0], [1, 1, 1, 1], [2, 2, 2, 2], [3, 3, 3, 3], [0, 1, 2, 3], [3, 2, 1, 1], [1, 0, -1, 2]):
+        out, out_lens, used = (x.cpu() for x in ops.beam_reorder(ints([parents]), table.cuda(), ints(lens), spare.cuda(),
+                                                                 kc.cuda(), vc.cuda()))
+        for r, p in enumerate(parents):
+            if p < 0:
+                assert (out[r] == -1).all()
+                continue
+            held, mine = -(-lens[p] // page), -(-lens[r] // page)
+            want = table[p, :held].tolist() + [-1] * (mine - held) + table[r, max(held, mine):].tolist()
+            copied = p in parents[:r] and lens[p] % page > 0
+            if copied:
+                want[held - 1] = int(spare[r])
+            assert out[r].tolist() == want and int(out_lens[r]) == lens[p] and int(used[r]) == copied
+        live = out[[p >= 0 for p in parents]]
+        behind = [int(x) for line, n in zip(live, out_lens[[p >= 0 for p in parents]]) for x in line[-(-int(n) // page):] if x >= 0]
+        assert len(behind) == len(set(behind))
+
+
+def test_beams_with_reserved_pages_write_apart():
+    """Three beams with 16-row pages reserved ahead go on from one of them, in the middle of a page and at its end: what
+    each appends afterwards is its own."""
+    page, d, beams, steps = 16, 64, 3, 40
+    width = -(-steps // page)
+    pages = beams * width + beams * steps
+    kc, vc = torch.zeros(pages, 1, page, d, dtype=F16).cuda(), torch.zeros(pages, 1, page, d, dtype=F16).cuda()
+    table, lens = torch.arange(beams * width, dtype=torch.int32).view(beams, width).cuda(), ints([0] * beams)
+    fresh = torch.arange(beams * width, pages, dtype=torch.int32).view(steps, beams).cuda()
+    freqs = torch.zeros(1, dtype=torch.float64).cuda()  # no rotation
+    history = [[] for _ in range(beams)]
+    for step in range(steps):
+        qkv = torch.zeros(beams, 3 * d)
+        qkv[:, 2 * d:] = (step * beams + torch.arange(beams, dtype=torch.float32))[:, None] / 8
+        ops.paged_qkv_append(qkv.cuda(), lens, lens, table, kc, vc, 1, freqs)
+        lens = lens + 1
+        history = [h + [(step * beams + i) / 8] for i, h in enumerate(history)]
+        parents = {7: [1, 1, 1], 15: [1, 1, 1], 20: [2, 0, 2], 31: [2, 2, 0]}.get(step, [0, 1, 2])
+        table, lens, _ = ops.beam_reorder(ints([parents]), table, lens, fresh[step], kc, vc)
+        history = [history[p] for p in parents]
+        for i in range(beams):
+            got = vc[table[i, :-(-(step + 1) // page)].long(), 0, :, 0].flatten()[:step + 1]
+            assert got.tolist() == history[i], (step, i)
