@@ -76,8 +76,8 @@ const char *mllb_last_error(void);
  * attention gave up waiting for its K/V copies; bit 6 = a peer all-gather
  * gave up waiting for another rank; bit 7 = a grid-wide epilogue
  * (mllb_q4k_matvec_norm) gave up waiting for the other CTAs of its grid;
- * bit 8 = a page, sequence or length of a paged cache outside its table or
- * cache; bit 9 = a beam's parent outside its batch entry.
+ * bit 8 = a page, sequence, length or start of a paged call outside its table,
+ * cache or call; bit 9 = a beam's parent outside its batch entry.
  * Copies the word of the current device to *bits (synchronising),
  * optionally clearing it.  0 in normal runs.
  */
@@ -579,7 +579,9 @@ int mllb_paged_qkv_append(const mllb_paged_append *args, const mllb_paged_cache 
  * also see all prefix_lens[g] rows of prefix_table[g]; a group's prefix is
  * read once for all its sequences where they have few tokens.  groups 0: no
  * prefixes; group_start NULL: one group of all sequences.  A token that sees
- * nothing gets zeros; tokens behind q_start[seqs] stay as they are.  Rows
+ * nothing gets zeros; tokens behind q_start[seqs] stay as they are.  q_start and
+ * group_start ascend within [0, tokens] and [0, seqs]: what lies outside counts
+ * as the end, where they descend out is of no use, both set bit 8.  Rows
  * behind a sequence's length may hold anything, NaN too; the visible ones,
  * and those of a sequence's later tokens, must be finite.  q head h reads KV
  * head h / (q_heads / kv_heads).  q and out have the cache's type, and out

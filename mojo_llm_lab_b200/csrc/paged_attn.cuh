@@ -58,8 +58,8 @@ struct AttnPass {
   int dense;       // 1: segment of CTA c and item i at slot c + i; 0: at 2 c (a CTA's first) or 2 c + 1
   int slots;       // capacity of the workspace
   int rows, keys;  // R and KT of the kernel that ran it (for the merge)
-  // For the kernel that joins.  dense: [entities] items before each entity,
-  // then int2 [items] first and last CTA of an item; otherwise AttnCut, the
+  // For the kernel that joins.  dense: [entities] items before each entity, 1
+  // (0: the starts descend, nothing was done), then int2 [items] first and last CTA of an item; otherwise AttnCut, the
   // number of records first (as segments), then one an item (by_item: there are
   // no more items than CTAs) or one a CTA.
   int32_t* plan;
@@ -76,7 +76,7 @@ struct AttnCut {
 };
 
 struct AttnEntity {
-  int tok0, ntok, plen, len, causal;
+  int tok0, ntok, plen, len, causal;  // ntok < 0: starts that descend (attn_start: no work at all)
   const int32_t* ptab;
   const int32_t* tab;
 };
@@ -111,7 +111,7 @@ __device__ __forceinline__ AttnEntity attn_entity(const AttnArgs& a, int mode, i
   if (mode == kAttnPrefix || (mode == kAttnBoth && e < a.groups)) {
     const int s0 = a.group_start ? a.group_start[e] : 0, s1 = a.group_start ? a.group_start[e + 1] : a.seqs;
     n.tok0 = attn_token_start(a, s0);
-    n.ntok = max(attn_token_start(a, s1) - n.tok0, 0);
+    n.ntok = attn_token_start(a, s1) - n.tok0;
     n.len = attn_clamp_len(a.prefix_lens[e], a.prefix_width, a.page_shift);
     n.tab = a.prefix_table + static_cast<long long>(e) * a.prefix_width;
     n.causal = 0;
@@ -119,7 +119,7 @@ __device__ __forceinline__ AttnEntity attn_entity(const AttnArgs& a, int mode, i
   }
   const int seq = mode == kAttnBoth ? e - a.groups : e;
   n.tok0 = attn_token_start(a, seq);
-  n.ntok = max(attn_token_start(a, seq + 1) - n.tok0, 0);
+  n.ntok = attn_token_start(a, seq + 1) - n.tok0;
   n.len = attn_clamp_len(a.lens[seq], a.width, a.page_shift);
   n.tab = a.table + static_cast<long long>(seq) * a.width;
   n.causal = 1;
@@ -173,13 +173,16 @@ struct AttnCursor {
   int item;        // number of the item on the line
 };
 
-// Entity e's length on the line (attn_cost of its items) and its items; 0 past the last.
+// Entity e's length on the line (attn_cost of its items) and its items; 0 past
+// the last.  False where its starts descend.
 template <int R, int KT>
-__device__ __forceinline__ void attn_work(const AttnArgs& a, const AttnPass& pass, int e, int* pairs, int* items) {
+__device__ __forceinline__ bool attn_work(const AttnArgs& a, const AttnPass& pass, int e, int* pairs, int* items) {
   int w = 0, t = 0;
+  bool ascends = true;
   if (e < pass.entities) {
     const AttnEntity ent = attn_entity(a, pass.mode, e);
-    t = attn_row_tiles(ent, a.ratio, R);
+    ascends = ent.ntok >= 0;
+    t = ascends ? attn_row_tiles(ent, a.ratio, R) : 0;
     if (ent.causal && ent.ntok > 1) {
       for (int i = 0; i < t; ++i) w += attn_cost(attn_key_tiles(ent, a.ratio, i, R, KT, !pass.dense), R);
     } else if (t > 0) {
@@ -188,6 +191,17 @@ __device__ __forceinline__ void attn_work(const AttnArgs& a, const AttnPass& pas
   }
   *pairs = w * a.kv_heads;
   *items = t * a.kv_heads;
+  return ascends;
+}
+
+// Starts outside the call's tokens or sequences count as their ends, and starts
+// that descend as no call; either is flagged.
+template <int kThreads>
+__device__ __forceinline__ void attn_check_starts(const AttnArgs& a) {
+  for (int i = threadIdx.x; a.q_start && i <= a.seqs; i += kThreads)
+    if (a.q_start[i] < (i ? max(a.q_start[i - 1], 0) : 0) || a.q_start[i] > a.tokens) record_error(kErrBadPage);
+  for (int i = threadIdx.x; a.group_start && i <= a.groups; i += kThreads)
+    if (a.group_start[i] < (i ? max(a.group_start[i - 1], 0) : 0) || a.group_start[i] > a.seqs) record_error(kErrBadPage);
 }
 
 // This CTA's share, which starts `rest` pairs into entity e (whose first item is `item0`).
@@ -220,14 +234,20 @@ __device__ __forceinline__ AttnCursor attn_locate(const AttnArgs& a, const AttnP
 // Adds up all entities' work and finds this CTA's share.  All threads of the
 // CTA call it; `scan` is shared scratch of 2 (entities + 1) + 64 ints.  CTA 0
 // leaves the numbers of items, or of records, in pass.plan.
+//
+// Starts that ascend share out the call's tokens, whatever their values, so the
+// sums stay below the 2^31 that the host has checked.  Descending ones count
+// tokens many times over, and a sum that wraps would send attn_locate after a
+// place that does not exist: then the pass has no work.
 template <int R, int KT, int kThreads>
 __device__ __forceinline__ AttnCursor attn_start(const AttnArgs& a, const AttnPass& pass, int* scan) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   constexpr int kWarps = kThreads / 32;
+  if (blockIdx.x == 0) attn_check_starts<kThreads>(a);
   if (pass.entities <= 32) {
     // Few entities: every warp adds them up for itself, a lane each.
     int w, n;
-    attn_work<R, KT>(a, pass, lane, &w, &n);
+    const bool ascends = __all_sync(0xffffffffu, attn_work<R, KT>(a, pass, lane, &w, &n));
     int ws = w, ns = n;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
@@ -235,10 +255,11 @@ __device__ __forceinline__ AttnCursor attn_start(const AttnArgs& a, const AttnPa
       if (lane >= d) ws += wu, ns += nu;
     }
     if (blockIdx.x == 0 && warp == 0) {
-      if (!pass.dense && lane == 31) pass.plan[0] = pass.by_item ? ns : pass.ctas;
+      if (!pass.dense && lane == 31) pass.plan[0] = !ascends ? 0 : pass.by_item ? ns : pass.ctas;
       if (pass.dense && lane < pass.entities) pass.plan[lane] = ns - n;
+      if (pass.dense && lane == 0) pass.plan[pass.entities] = ascends;
     }
-    const int total = __shfl_sync(0xffffffffu, ws, 31), ctas = min(pass.ctas, total);
+    const int total = ascends ? __shfl_sync(0xffffffffu, ws, 31) : 0, ctas = min(pass.ctas, total);
     const int w0 = attn_share(total, max(ctas, 1), blockIdx.x);
     // The entity that holds pair w0: the first whose sum passes it.
     const unsigned past = __ballot_sync(0xffffffffu, ws > w0);
@@ -248,10 +269,10 @@ __device__ __forceinline__ AttnCursor attn_start(const AttnArgs& a, const AttnPa
   int* tiles = scan;
   int* items = scan + pass.entities + 1;
   int* part = items + pass.entities + 1;  // [2][kWarps]
-  int tiles_before = 0, items_before = 0;
+  int tiles_before = 0, items_before = 0, descends = 0;
   for (int e0 = 0; e0 < pass.entities; e0 += kThreads) {
     int w, n;
-    attn_work<R, KT>(a, pass, e0 + tid, &w, &n);
+    const bool ascends = attn_work<R, KT>(a, pass, e0 + tid, &w, &n);
     int ws = w, ns = n;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
@@ -259,7 +280,7 @@ __device__ __forceinline__ AttnCursor attn_start(const AttnArgs& a, const AttnPa
       if (lane >= d) ws += wu, ns += nu;
     }
     if (lane == 31) part[warp] = ws, part[kWarps + warp] = ns;
-    __syncthreads();
+    descends |= __syncthreads_or(!ascends);
     int wb = tiles_before, nb = items_before;
     for (int i = 0; i < kWarps; ++i) {
       if (i < warp) wb += part[i], nb += part[kWarps + i];
@@ -278,10 +299,11 @@ __device__ __forceinline__ AttnCursor attn_start(const AttnArgs& a, const AttnPa
   }
   __syncthreads();
   if (blockIdx.x == 0) {
-    if (!pass.dense && tid == 0) pass.plan[0] = pass.by_item ? items_before : pass.ctas;
+    if (!pass.dense && tid == 0) pass.plan[0] = descends ? 0 : pass.by_item ? items_before : pass.ctas;
     if (pass.dense)
-      for (int i = tid; i < pass.entities; i += kThreads) pass.plan[i] = items[i];
+      for (int i = tid; i <= pass.entities; i += kThreads) pass.plan[i] = i < pass.entities ? items[i] : !descends;
   }
+  if (descends) return {};
   const int w0 = attn_share(tiles_before, max(min(pass.ctas, tiles_before), 1), blockIdx.x);
   int lo = 0, hi = pass.entities;  // tiles[lo] <= w0 < tiles[hi]
   while (hi - lo > 1) {
@@ -785,10 +807,10 @@ __device__ __forceinline__ AttnRowParts attn_row_parts(const AttnArgs& a, const 
   if (attn_key_tiles(ent, a.ratio, t, pass.rows, pass.keys, 0) == 0) return p;
   p.row = row - t * pass.rows;
   p.item = before + t * a.kv_heads + h;
-  if (p.item >= pass.slots) return p;
+  if (p.item < 0 || p.item >= pass.slots) return p;
   const int2 ctas = reinterpret_cast<const int2*>(pass.plan + (pass.entities + 2) / 2 * 2)[p.item];
-  p.c0 = max(ctas.x, 0);
-  p.c1 = min(ctas.y, pass.ctas - 1);
+  p.c1 = max(min(ctas.y, pass.ctas - 1), -1);
+  p.c0 = min(max(ctas.x, 0), p.c1 + 1);
   return p;
 }
 
@@ -945,6 +967,7 @@ __global__ void __launch_bounds__(256)
     seq = lo;
   }
   AttnJoin<D> join;
+  const bool done = first.plan[first.entities] && (first.mode == kAttnBoth || second.plan[second.entities]);
   if (there) {
     const int g = attn_group_of(a, seq);
     AttnRowParts pre = {0, -1, 0, 0};
@@ -958,7 +981,7 @@ __global__ void __launch_bounds__(256)
                                  : attn_slot<D>(own_pass, own.c0 + i - shared_segments + own.item, own.row);
     });
   }
-  if (!join.gather(shared, warp, lane, part, parts) || !there) return;
+  if (!join.gather(shared, warp, lane, part, parts) || !there || !done) return;
   attn_store_row<D, kBf16>(a, token, head, lane, join.sum, join.acc);
 }
 

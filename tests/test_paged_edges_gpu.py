@@ -131,3 +131,62 @@ def test_beams_with_reserved_pages_write_apart():
         for i in range(beams):
             got = vc[table[i, :-(-(step + 1) // page)].long(), 0, :, 0].flatten()[:step + 1]
             assert got.tolist() == history[i], (step, i)
+
+
+# ------------------------------------------------------------------ starts that make no sense
+
+# One call of each kind of plan: (lens, news, prefix, wide prefix table): items by number, items by CTA, more than 32
+# sequences, prefixes and own rows in one pass, prefixes in a pass of their own, in one on the tensor cores.
+PLANS = [([90, 200, 30], [3, 7, 5], [], False), ([90, 200, 30], [40, 170, 25], [], False),
+         ([300] * 60, [100] * 60, [200], False), ([64] * 40, [2] * 40, [], False), ([90, 40, 30], [3, 2, 1], [64], True),
+         ([9] * 50, [1] * 50, [64], True), ([90, 40, 30], [9, 2, 5], [64], True), ([9] * 80, [3] * 80, [640], True)]
+
+
+def guarded(count, dtype, fill):
+    """A tensor of `count` elements with 4096 more on both sides, and a check that those are as they were."""
+    whole = torch.full((count + 8192,), fill, dtype=dtype, device="cuda")
+    return whole[4096:-4096], lambda: bool((whole[:4096] == fill).all() and (whole[-4096:] == fill).all())
+
+
+@pytest.mark.parametrize("lens,news,prefix,wide", PLANS)
+@pytest.mark.parametrize("what", ["good", "descending", "repeating", "behind", "negative", "groups descend", "groups behind"])
+def test_starts_stay_inside(lens, news, prefix, wide, what):
+    hq, hk, d, page, seqs, tokens = 8, 2, 128, 16, len(lens), sum(news)
+    if "groups" in what and not prefix:
+        return
+    table, pages, _ = P.tables(lens + prefix * 2, page, 3)
+    kc, vc = (x.cuda() for x in P.cache(pages, hk, page, d, F16, 5))
+    q = torch.randn(tokens, hq, d, generator=torch.Generator().manual_seed(1)).to(F16).cuda()
+    starts = [0] + torch.tensor(news).cumsum(0).tolist()
+    groups = [0, seqs // 2, seqs]
+    if what == "descending":
+        starts[1:-1] = starts[1:-1][::-1]
+    elif what == "repeating":  # every second sequence has all tokens
+        starts = [i % 2 * tokens for i in range(seqs + 1)]
+    elif what == "behind":
+        starts[-1] = 10 ** 6
+    elif what == "negative":
+        starts[0] = -3
+    elif what == "groups descend":
+        groups = [seqs, 0, seqs]
+    elif what == "groups behind":
+        groups[-1] = 10 ** 6
+    more = dict(q_start=ints(starts))
+    if prefix:
+        lines = table[seqs:, :-(-prefix[0] // page)]
+        if wide:  # so wide that the prefixes run once a group
+            lines = torch.cat([lines, torch.full((2, 192 * 2 ** 20 // ((seqs - 2) * page * hk * d * 4) + 1), -1)], 1)
+        more.update(prefix_table=lines.to(torch.int32).contiguous().cuda(), prefix_lens=ints(prefix * 2), group_start=ints(groups))
+    need = ops.paged_attention_workspace(tokens, hq, hk, d, seqs, 2 if prefix else 0, "cuda").numel()
+    work, work_whole = guarded(need, torch.uint8, 171)
+    out, out_whole = guarded(tokens * hq * d, F16, 7.0)
+    out = out.view(tokens, hq, d)
+    ops.paged_attention(q, kc, vc, table[:seqs, :-(-max(lens) // page)].contiguous().cuda(), ints(lens), out=out,
+                        workspace=work, **more)
+    torch.cuda.synchronize()
+    assert work_whole() and out_whole()
+    assert ops.device_error() == (0 if what == "good" else BAD_PAGE)
+    if what in ("descending", "repeating"):
+        assert (out == 7.0).all()
+    elif what != "groups descend":
+        assert torch.isfinite(out).all() and not (out[starts[1]:] == 7.0).all(-1).any()
