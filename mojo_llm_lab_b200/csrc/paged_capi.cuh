@@ -21,6 +21,16 @@ int log2_exact(int64_t n) {
   return s;
 }
 
+// Whether two of the rows of d elements at t * token + h * head, t < tokens, h < heads, have an element in common.
+bool rows_overlap(int64_t tokens, int64_t token, int64_t heads, int64_t head, int64_t d) {
+  if (tokens > 1 && token < d) return true;
+  for (int64_t h = 1; h < heads; ++h) {  // row (0, h) lies between rows (t, 0) and (t + 1, 0), or behind all
+    const int64_t at = h * head, t = tokens > 1 ? at / token : 0, behind = at - t * token;
+    if ((t < tokens && behind < d) || (t + 1 < tokens && token - behind < d)) return true;
+  }
+  return false;
+}
+
 // Checks a cache description and turns it into the kernels' form.
 int paged_cache(const mllb_paged_cache* c, mllb::PagedCache* out) {
   if (!c || !c->k || !c->v) return fail(MLLB_EINVAL, "null pointer: cache");
@@ -432,7 +442,9 @@ int mllb_paged_attention(const mllb_paged_attn* p, const mllb_paged_cache* cache
   const int64_t strides[4] = {p->q_token_stride, p->q_head_stride, p->out_token_stride, p->out_head_stride};
   for (int64_t s : strides)
     if (s < 0 || s % 8) return fail(MLLB_EALIGN, "q and out strides must be multiples of 8 elements (16 bytes)");
-  if ((p->tokens > 1 && p->out_token_stride < cache->head_dim) || (p->q_heads > 1 && p->out_head_stride < cache->head_dim))
+  for (int64_t s : strides)
+    if (s >= (1ll << 38)) return fail(MLLB_EINVAL, "q and out strides must be below 2^38 elements");
+  if (rows_overlap(p->tokens, p->out_token_stride, p->q_heads, p->out_head_stride, cache->head_dim))
     return fail(MLLB_EINVAL, "rows of out overlap");
   if (!aligned(p->q, 16) || !aligned(p->out, 16) || !aligned(workspace, 16))
     return fail(MLLB_EALIGN, "q, out and workspace must be 16-byte aligned");

@@ -1,0 +1,26 @@
+"""Calls of the paged-cache operators whose results would race with what other CTAs read, or whose sizes do not fit:
+refused by the C entries before they touch CUDA (made-up addresses are never read)."""
+import pytest
+
+from mojo_llm_lab_b200 import _lib
+
+EINVAL = _lib.MLLB_EINVAL
+
+
+def cache(**kw):
+    return _lib.PagedCache(**{**dict(k=1 << 40, v=2 << 40, pages=4, kv_heads=2, page_size=16, head_dim=128, page_stride=4096,
+                                     head_stride=2048, row_stride=128, layers=1, layer_stride=0, type=_lib.TYPE_F16), **kw})
+
+
+def attend(workspace_bytes=1 << 40, **kw):
+    """3 tokens of 4 heads of 128: rows of 256 bytes."""
+    args = _lib.PagedAttn(**{**dict(q=1 << 20, out=1 << 30, tokens=3, q_heads=4, q_token_stride=512, q_head_stride=128,
+                                    out_token_stride=512, out_head_stride=128, page_table=4096, seq_lens=8192, seqs=3,
+                                    table_width=2, scale=0.1), **kw})
+    return _lib.lib().mllb_paged_attention(args, cache(), 1 << 41, workspace_bytes, 0, None)
+
+
+@pytest.mark.parametrize("token,head", [(128, 128), (256, 128), (128, 256), (384, 128), (320, 192), (512, 160), (136, 128)])
+def test_rows_of_out_over_one_another(token, head):
+    assert attend(out_token_stride=token, out_head_stride=head) == EINVAL
+    assert b"overlap" in _lib.lib().mllb_last_error()
