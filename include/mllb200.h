@@ -585,7 +585,7 @@ int mllb_paged_qkv_append(const mllb_paged_append *args, const mllb_paged_cache 
  * behind a sequence's length may hold anything, NaN too; the visible ones,
  * and those of a sequence's later tokens, must be finite.  q head h reads KV
  * head h / (q_heads / kv_heads).  q and out have the cache's type, and out
- * may be q itself; fp32 softmax and sums, the weights rounded to the cache's
+ * may be q itself (with its strides) but share no other rows with it; fp32 softmax and sums, the weights rounded to the cache's
  * type for the products with V.  workspace: mllb_paged_attention_workspace bytes (the number
  * depends on the current device), 16-byte aligned, any contents; calls that
  * share it must not overlap on the GPU.  seqs + groups <= 2048.

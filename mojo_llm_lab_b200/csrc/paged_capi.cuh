@@ -3,6 +3,8 @@
 // included by capi.cu behind its helpers.
 #pragma once
 
+#include <algorithm>
+
 #include "beam.cuh"
 #include "paged.cuh"
 #include "paged_attn.cuh"
@@ -28,6 +30,36 @@ bool rows_overlap(int64_t tokens, int64_t token, int64_t heads, int64_t head, in
     const int64_t at = h * head, t = tokens > 1 ? at / token : 0, behind = at - t * token;
     if ((t < tokens && behind < d) || (t + 1 < tokens && token - behind < d)) return true;
   }
+  return false;
+}
+
+// Whether a row of out has an element in common with a row of q, both of d
+// elements at t * token + h * head from their bases.  Rows of one buffer taken
+// in turn have the same token stride; with others, rows in the same range count
+// as shared.
+bool out_overlaps_q(const mllb_paged_attn* p, int64_t d) {
+  const int64_t tokens = p->tokens - 1, heads = p->q_heads - 1;
+  const auto q = reinterpret_cast<uintptr_t>(p->q), out = reinterpret_cast<uintptr_t>(p->out);
+  const uintptr_t q_end = q + 2 * (tokens * p->q_token_stride + heads * p->q_head_stride + d);
+  const uintptr_t out_end = out + 2 * (tokens * p->out_token_stride + heads * p->out_head_stride + d);
+  if (q_end <= out || out_end <= q) return false;
+  if (tokens && p->q_token_stride != p->out_token_stride) return true;
+  const int64_t base = (static_cast<int64_t>(out) - static_cast<int64_t>(q)) / 2, token = tokens ? p->out_token_stride : 0;
+  // Whether rows that lie x apart, or whole token strides more or less, meet.
+  auto meet = [&](int64_t x) {
+    const int64_t near = tokens ? std::min(std::max(x / token, -tokens), tokens) : 0;
+    for (int64_t t = std::max(near - 1, -tokens); t <= std::min(near + 1, tokens); ++t)
+      if (x - t * token > -d && x - t * token < d) return true;
+    return false;
+  };
+  if (heads == 0 || p->q_head_stride == p->out_head_stride) {
+    for (int64_t h = -heads; h <= heads; ++h)
+      if (meet(base + h * p->out_head_stride)) return true;
+    return false;
+  }
+  for (int64_t h = 0; h <= heads; ++h)
+    for (int64_t g = 0; g <= heads; ++g)
+      if (meet(base + h * p->out_head_stride - g * p->q_head_stride)) return true;
   return false;
 }
 
@@ -448,6 +480,10 @@ int mllb_paged_attention(const mllb_paged_attn* p, const mllb_paged_cache* cache
     return fail(MLLB_EINVAL, "rows of out overlap");
   if (!aligned(p->q, 16) || !aligned(p->out, 16) || !aligned(workspace, 16))
     return fail(MLLB_EALIGN, "q, out and workspace must be 16-byte aligned");
+  const bool in_place = p->q == p->out && (p->tokens == 1 || p->q_token_stride == p->out_token_stride) &&
+                        (p->q_heads == 1 || p->q_head_stride == p->out_head_stride);
+  if (!in_place && out_overlaps_q(p, cache->head_dim))
+    return fail(MLLB_EINVAL, "out must be q or must not overlap its rows");
   int dev;
   if ((rc = current_device(&dev))) return rc;
   PagedPlan plan;

@@ -780,7 +780,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     read once for all of a group's sequences.  A token that sees nothing gets zeros; tokens behind q_start[-1] are left
     as they are.  What a row's mask hides may hold anything behind a sequence's length; rows that later tokens of the
     sequence see must be finite.  At most 2048 sequences and groups.  scale: 1 / sqrt(head_dim) unless given.  out may
-    be q."""
+    be q, or must share no rows with it."""
     return native().paged_attention(q, k_cache, v_cache, page_table, seq_lens, prefix_table, prefix_lens, group_start,
                                     q_start, scale, out, workspace, pdl)
 

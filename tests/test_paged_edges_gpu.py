@@ -190,3 +190,22 @@ def test_starts_stay_inside(lens, news, prefix, wide, what):
         assert (out == 7.0).all()
     elif what != "groups descend":
         assert torch.isfinite(out).all() and not (out[starts[1]:] == 7.0).all(-1).any()
+
+
+# ------------------------------------------------------------------ results beside their inputs
+
+@pytest.mark.parametrize("tokens", [3, 200])
+def test_out_between_the_rows_of_q(tokens):
+    """q and out as interleaved views of one buffer: by token, by head, and rows one after the other."""
+    lens, page, hq, hk, d = [tokens], 16, 8, 2, 128
+    table, pages, _ = P.tables(lens, page, 3)
+    kc, vc = (x.cuda() for x in P.cache(pages, hk, page, d, F16, 5))
+    q = torch.randn(tokens, hq, d, generator=torch.Generator().manual_seed(1)).to(F16).cuda()
+    args = (kc, vc, table.cuda(), ints(lens))
+    want = ops.paged_attention(q, *args, q_start=ints([0, tokens]))
+    for shape, at in (((tokens, 2, hq, d), 1), ((tokens, hq, 2, d), 2), ((2, tokens, hq, d), 0), ((tokens, 2, hq, d), 1)):
+        buffer = torch.full(shape, 7.0, dtype=F16, device="cuda")
+        mine, out = buffer.select(at, 0), buffer.select(at, 1)
+        mine.copy_(q)
+        assert ops.paged_attention(mine, *args, q_start=ints([0, tokens]), out=out) is out
+        assert torch.equal(out, want) and torch.equal(mine, q)

@@ -24,3 +24,17 @@ def attend(workspace_bytes=1 << 40, **kw):
 def test_rows_of_out_over_one_another(token, head):
     assert attend(out_token_stride=token, out_head_stride=head) == EINVAL
     assert b"overlap" in _lib.lib().mllb_last_error()
+
+
+@pytest.mark.parametrize("kw", [
+    dict(out=(1 << 20) + 1024),                         # a token further on
+    dict(out=(1 << 20) - 256),                          # a head before
+    dict(out=(1 << 20) + 128),                          # half a row further on
+    dict(out_token_stride=1024), dict(out_head_stride=256, out_token_stride=1024),  # its first row, then others
+    dict(out_token_stride=128, out_head_stride=512),    # tokens and heads exchanged
+    dict(q_token_stride=0),                             # one query for all tokens, its rows over the first result's
+    dict(q_token_stride=1024, out_token_stride=1024, out=(1 << 20) + 512),  # the heads after the first two
+])
+def test_out_partly_over_q(kw):
+    assert attend(**{**dict(out=1 << 20), **kw}) == EINVAL
+    assert b"overlap" in _lib.lib().mllb_last_error()
