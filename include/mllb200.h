@@ -640,8 +640,8 @@ int mllb_beam_select(const mllb_beam_scores *args, float *out_scores, int32_t *o
  * the rows held copied for K and V of all layers; used[r] = 1 where fresh[r]
  * was taken.  fresh: distinct pages that no table line names.  A negative
  * parent ends the row (length 0, table -1, reserved pages too), one past the beams also sets
- * device error bit 9 (mask 0x200).  table_out and lens_out must not overlap
- * the inputs.
+ * device error bit 9 (mask 0x200).  table_out, lens_out and used must not
+ * overlap the inputs or one another.
  */
 typedef struct mllb_beam_rows {
     const int32_t *parents, *page_table, *seq_lens, *fresh;

@@ -23,6 +23,16 @@ int log2_exact(int64_t n) {
   return s;
 }
 
+// Memory that a call reads or writes.
+struct Span {
+  const void* at;
+  int64_t bytes;
+};
+bool meet(const Span& a, const Span& b) {
+  const auto x = reinterpret_cast<uintptr_t>(a.at), y = reinterpret_cast<uintptr_t>(b.at);
+  return x < y + b.bytes && y < x + a.bytes;
+}
+
 // Whether two of the rows of d elements at t * token + h * head, t < tokens, h < heads, have an element in common.
 bool rows_overlap(int64_t tokens, int64_t token, int64_t heads, int64_t head, int64_t d) {
   if (tokens > 1 && token < d) return true;
@@ -46,7 +56,7 @@ bool out_overlaps_q(const mllb_paged_attn* p, int64_t d) {
   if (tokens && p->q_token_stride != p->out_token_stride) return true;
   const int64_t base = (static_cast<int64_t>(out) - static_cast<int64_t>(q)) / 2, token = tokens ? p->out_token_stride : 0;
   // Whether rows that lie x apart, or whole token strides more or less, meet.
-  auto meet = [&](int64_t x) {
+  auto near_zero = [&](int64_t x) {
     const int64_t near = tokens ? std::min(std::max(x / token, -tokens), tokens) : 0;
     for (int64_t t = std::max(near - 1, -tokens); t <= std::min(near + 1, tokens); ++t)
       if (x - t * token > -d && x - t * token < d) return true;
@@ -54,12 +64,12 @@ bool out_overlaps_q(const mllb_paged_attn* p, int64_t d) {
   };
   if (heads == 0 || p->q_head_stride == p->out_head_stride) {
     for (int64_t h = -heads; h <= heads; ++h)
-      if (meet(base + h * p->out_head_stride)) return true;
+      if (near_zero(base + h * p->out_head_stride)) return true;
     return false;
   }
   for (int64_t h = 0; h <= heads; ++h)
     for (int64_t g = 0; g <= heads; ++g)
-      if (meet(base + h * p->out_head_stride - g * p->q_head_stride)) return true;
+      if (near_zero(base + h * p->out_head_stride - g * p->q_head_stride)) return true;
   return false;
 }
 
@@ -629,13 +639,14 @@ int mllb_beam_reorder(const mllb_beam_rows* p, const mllb_paged_cache* cache, in
   if (p->batch <= 0 || p->beams <= 0 || p->batch * p->beams > 65535) return fail(MLLB_EINVAL, "batch x beams out of range");
   if (p->table_width <= 0 || p->table_width > (1 << 24)) return fail(MLLB_EINVAL, "table width out of range");
   const int64_t rows = p->batch * p->beams;
-  const struct { const void* in; int64_t in_bytes; const void* out; int64_t out_bytes; } pairs[] = {
-      {p->page_table, rows * p->table_width * 4, table_out, rows * p->table_width * 4},
-      {p->seq_lens, rows * 4, lens_out, rows * 4}};
-  for (const auto& q : pairs) {
-    const auto i = reinterpret_cast<uintptr_t>(q.in), o = reinterpret_cast<uintptr_t>(q.out);
-    if (i < o + q.out_bytes && o < i + q.in_bytes)
-      return fail(MLLB_EINVAL, "the reordered table and lengths must not overlap those they come from");
+  // Rows are written while others' parents, lines, lengths and fresh pages are still read.
+  const Span in[] = {{p->parents, rows * 4}, {p->page_table, rows * p->table_width * 4}, {p->seq_lens, rows * 4}, {p->fresh, rows * 4}};
+  const Span out[] = {{table_out, rows * p->table_width * 4}, {lens_out, rows * 4}, {used, rows * 4}};
+  for (int i = 0; i < 3; ++i) {
+    for (const Span& s : in)
+      if (meet(out[i], s)) return fail(MLLB_EINVAL, "the reordered table, lengths and used must not overlap what they come from");
+    for (int j = 0; j < i; ++j)
+      if (meet(out[i], out[j])) return fail(MLLB_EINVAL, "the reordered table, lengths and used must not overlap one another");
   }
   if (!aligned(p->parents, 4) || !aligned(p->page_table, 4) || !aligned(p->seq_lens, 4) || !aligned(p->fresh, 4) ||
       !aligned(table_out, 4) || !aligned(lens_out, 4) || !aligned(used, 4))

@@ -38,3 +38,26 @@ def test_rows_of_out_over_one_another(token, head):
 def test_out_partly_over_q(kw):
     assert attend(**{**dict(out=1 << 20), **kw}) == EINVAL
     assert b"overlap" in _lib.lib().mllb_last_error()
+
+
+@pytest.mark.parametrize("over", ["parents", "page_table", "seq_lens", "fresh"])
+@pytest.mark.parametrize("which", [0, 1, 2])
+@pytest.mark.parametrize("where", ["same", "first", "last"])
+def test_reorder_into_what_it_reads(over, which, where):
+    """2 x 4 rows of 3 pages: lists of 32 bytes, tables of 96."""
+    places = dict(parents=1 << 20, page_table=2 << 20, seq_lens=3 << 20, fresh=4 << 20)
+    out, sizes = [5 << 20, 6 << 20, 7 << 20], [96, 32, 32]
+    read = 96 if over == "page_table" else 32
+    out[which] = places[over] + {"same": 0, "first": read - 4, "last": 4 - sizes[which]}[where]
+    args = _lib.BeamRows(**places, batch=2, beams=4, table_width=3)
+    assert _lib.lib().mllb_beam_reorder(args, cache(), *out, 0, None) == EINVAL
+    assert b"overlap" in _lib.lib().mllb_last_error()
+
+
+@pytest.mark.parametrize("which,by", [((0, 1), 0), ((0, 2), 92), ((1, 2), 28)])
+def test_reorder_results_over_one_another(which, by):
+    out = [5 << 20, 6 << 20, 7 << 20]
+    out[which[1]] = out[which[0]] + by
+    args = _lib.BeamRows(1 << 20, 2 << 20, 3 << 20, 4 << 20, 2, 4, 3)
+    assert _lib.lib().mllb_beam_reorder(args, cache(), *out, 0, None) == EINVAL
+    assert b"overlap" in _lib.lib().mllb_last_error()
