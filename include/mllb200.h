@@ -616,7 +616,9 @@ int mllb_paged_attention(const mllb_paged_attn *args, const mllb_paged_cache *ca
  * -inf, +inf as the largest finite fp32.  A logit of -inf is no candidate;
  * a done beam's only candidate is end_token at the beam's score.  Places
  * without a candidate: -inf, -1, -1.  beams and n at most 64, vocab at most
- * 2^26.  Scores are compared in fp64.  workspace as for the attention.
+ * 2^26.  Scores are compared in fp64.  workspace as for the attention.  Results
+ * must not overlap one another, scores, done or the workspace, except that
+ * out_scores may be scores where n is beams.
  */
 typedef struct mllb_beam_scores {
     const void *logits; /* [batch][beams][vocab], strides in elements */

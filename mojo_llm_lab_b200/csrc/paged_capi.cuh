@@ -588,6 +588,17 @@ int mllb_beam_select(const mllb_beam_scores* p, float* out_scores, int32_t* out_
   if (workspace_bytes < need)
     return fail(MLLB_EINVAL, "workspace of %lld bytes, %lld needed", static_cast<long long>(workspace_bytes),
                 static_cast<long long>(need));
+  // An entry's results are written while other entries' scores, sums and lists are still read.
+  const int64_t rows = p->batch * p->beams, picked = p->batch * p->n * 4;
+  const Span in[] = {{p->scores, rows * 4}, {p->done ? p->done : workspace, p->done ? rows : 1}, {workspace, need}};
+  const Span out[] = {{out_scores, picked}, {out_tokens, picked}, {out_parents, picked}};
+  for (int i = 0; i < 3; ++i) {
+    for (const Span& s : in)
+      if (meet(out[i], s) && !(i == 0 && out_scores == p->scores && s.at == p->scores && p->n == p->beams))
+        return fail(MLLB_EINVAL, "results must not overlap scores (but be them, where n is beams), done or the workspace");
+    for (int j = 0; j < i; ++j)
+      if (meet(out[i], out[j])) return fail(MLLB_EINVAL, "results must not overlap one another");
+  }
   mllb::BeamArgs a = {};
   a.logits = p->logits;
   a.scores = p->scores;
@@ -606,7 +617,7 @@ int mllb_beam_select(const mllb_beam_scores* p, float* out_scores, int32_t* out_
   // 11 us, with one CTA for 36 steps of a row 23).
   int dev;
   if ((rc = current_device(&dev))) return rc;
-  const int64_t steps = beam_steps(p->vocab), rows = p->batch * p->beams;
+  const int64_t steps = beam_steps(p->vocab);
   int64_t chunks = 4ll * sm_count(dev) / rows;
   if (chunks < 1) chunks = 1;
   a.steps = static_cast<int>((steps + chunks - 1) / chunks);

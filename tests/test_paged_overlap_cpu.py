@@ -61,3 +61,23 @@ def test_reorder_results_over_one_another(which, by):
     args = _lib.BeamRows(1 << 20, 2 << 20, 3 << 20, 4 << 20, 2, 4, 3)
     assert _lib.lib().mllb_beam_reorder(args, cache(), *out, 0, None) == EINVAL
     assert b"overlap" in _lib.lib().mllb_last_error()
+
+
+def select(n=4, batch=3, out=(5 << 20, 6 << 20, 7 << 20), workspace=8 << 20, **kw):
+    """batch entries of 4 beams: scores of 48 bytes, results of 12 n."""
+    args = _lib.BeamScores(**{**dict(logits=1 << 20, batch=batch, beams=4, vocab=1000, n=n, batch_stride=4000, beam_stride=1000,
+                                     scores=2 << 20, done=3 << 20, end_token=1), **kw})
+    return _lib.lib().mllb_beam_select(args, *out, workspace, 1 << 20, 0, None)
+
+
+@pytest.mark.parametrize("n,which,place", [
+    (5, 0, 2 << 20), (3, 0, 2 << 20), (4, 0, (2 << 20) + 16), (4, 0, (2 << 20) - 44),  # one entry's results, another's scores
+    (4, 1, 2 << 20), (4, 2, (2 << 20) + 44),                        # tokens and parents over scores
+    (4, 0, 3 << 20), (4, 1, (3 << 20) + 8), (4, 2, (3 << 20) - 44),  # over done
+    (4, 0, 8 << 20), (4, 1, (8 << 20) + 64),                        # over the workspace
+    (4, 1, 5 << 20), (4, 2, (6 << 20) + 44)])                       # over one another
+def test_select_into_what_it_reads(n, which, place):
+    out = [5 << 20, 6 << 20, 7 << 20]
+    out[which] = place
+    assert select(n, out=out) == EINVAL
+    assert b"overlap" in _lib.lib().mllb_last_error()
