@@ -125,8 +125,8 @@ int check_beams(int64_t batch, int64_t beams, int64_t vocab, int64_t n) {
   if (beams > mllb::kBeamMost || n > mllb::kBeamMost)
     return fail(MLLB_EUNSUPPORTED, "at most %d beams and candidates", mllb::kBeamMost);
   if (vocab > (1ll << mllb::kBeamTokenBits)) return fail(MLLB_EINVAL, "vocab above 2^%d", mllb::kBeamTokenBits);
+  if (batch > 65535 || batch * beams > 65535) return fail(MLLB_EINVAL, "batch x beams above 65535");
   if (n > beams * vocab) return fail(MLLB_EINVAL, "n above beams x vocab: out of range");
-  if (batch * beams > 65535) return fail(MLLB_EINVAL, "batch x beams above 65535");
   return MLLB_OK;
 }
 
@@ -277,7 +277,7 @@ int check_attn_sizes(int64_t tokens, int64_t q_heads, int64_t kv_heads, int64_t 
   if (q_heads > 1024 || tokens > (1 << 24) || tokens * q_heads >= (1ll << 31))
     return fail(MLLB_EINVAL, "q_heads or tokens out of range");
   if (groups > seqs) return fail(MLLB_EINVAL, "more groups than sequences");
-  if (seqs + groups > mllb::kAttnMaxEntities)
+  if (seqs > mllb::kAttnMaxEntities || seqs + groups > mllb::kAttnMaxEntities)
     return fail(MLLB_EUNSUPPORTED, "more than %d sequences and groups", mllb::kAttnMaxEntities);
   return MLLB_OK;
 }
@@ -399,6 +399,7 @@ int mllb_paged_qkv_append(const mllb_paged_append* p, const mllb_paged_cache* ca
   if (p->rot_dim < 2 || p->rot_dim > d || p->rot_dim % 2)
     return fail(MLLB_EINVAL, "rot_dim=%lld is not an even number from 2 to head_dim", static_cast<long long>(p->rot_dim));
   const int64_t heads = p->q_heads + 2 * cache->kv_heads, size = p->qkv_type == MLLB_TYPE_F32 ? 4 : 2;
+  if (p->tokens > 1 && p->qkv_stride >= (1ll << 38)) return fail(MLLB_EINVAL, "qkv_stride must be below 2^38 elements");
   if (p->tokens > 1 && p->qkv_stride < heads * d) return fail(MLLB_EINVAL, "qkv rows overlap");
   if (!aligned(p->qkv, 16) || (p->qkv_stride * size) % 16) return fail(MLLB_EALIGN, "qkv rows must be 16-byte aligned");
   if (!aligned(p->q_out, 8) || !aligned(p->freqs, 8) || !aligned(p->positions, 4) || !aligned(p->rows, 4) ||
@@ -478,7 +479,7 @@ int mllb_paged_attention(const mllb_paged_attn* p, const mllb_paged_cache* cache
   if (p->groups > 1 && !p->group_start) return fail(MLLB_EINVAL, "null pointer: group_start (needed for several groups)");
   if (!p->q_start && p->tokens != p->seqs) return fail(MLLB_EINVAL, "without q_start every sequence has one token");
   if (p->table_width <= 0 || (p->groups && p->prefix_width <= 0)) return fail(MLLB_EINVAL, "page tables need a width");
-  if (p->table_width * cache->page_size >= (1ll << 30) || p->prefix_width * cache->page_size >= (1ll << 30))
+  if (p->table_width >= (1 << 30) / cache->page_size || (p->groups && p->prefix_width >= (1 << 30) / cache->page_size))
     return fail(MLLB_EINVAL, "page tables of 2^30 rows or more");
   if (!(p->scale == p->scale) || p->scale - p->scale != 0.0) return fail(MLLB_EINVAL, "scale must be finite");
   const int64_t strides[4] = {p->q_token_stride, p->q_head_stride, p->out_token_stride, p->out_head_stride};
@@ -583,7 +584,8 @@ int mllb_beam_select(const mllb_beam_scores* p, float* out_scores, int32_t* out_
   if (!aligned(p->logits, size) || !aligned(p->scores, 4) || !aligned(out_scores, 4) || !aligned(out_tokens, 4) ||
       !aligned(out_parents, 4) || !aligned(workspace, 16))
     return fail(MLLB_EALIGN, "workspace needs 16-byte, the other pointers their type's alignment");
-  if (p->batch_stride < 0 || p->beam_stride < 0) return fail(MLLB_EINVAL, "strides must not be negative");
+  if (p->batch_stride < 0 || p->beam_stride < 0 || p->batch_stride >= (1ll << 38) || p->beam_stride >= (1ll << 38))
+    return fail(MLLB_EINVAL, "strides must not be negative, and below 2^38 elements");
   const int64_t need = mllb_beam_select_workspace(p->batch, p->beams, p->vocab, p->n);
   if (workspace_bytes < need)
     return fail(MLLB_EINVAL, "workspace of %lld bytes, %lld needed", static_cast<long long>(workspace_bytes),
@@ -647,7 +649,8 @@ int mllb_beam_reorder(const mllb_beam_rows* p, const mllb_paged_cache* cache, in
   mllb::ReorderArgs a = {};
   const int rc = paged_cache(cache, &a.cache);
   if (rc) return rc;
-  if (p->batch <= 0 || p->beams <= 0 || p->batch * p->beams > 65535) return fail(MLLB_EINVAL, "batch x beams out of range");
+  if (p->batch <= 0 || p->beams <= 0 || p->batch > 65535 || p->beams > 65535 || p->batch * p->beams > 65535)
+    return fail(MLLB_EINVAL, "batch x beams out of range");
   if (p->table_width <= 0 || p->table_width > (1 << 24)) return fail(MLLB_EINVAL, "table width out of range");
   const int64_t rows = p->batch * p->beams;
   // Rows are written while others' parents, lines, lengths and fresh pages are still read.

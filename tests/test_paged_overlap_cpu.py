@@ -81,3 +81,20 @@ def test_select_into_what_it_reads(n, which, place):
     out[which] = place
     assert select(n, out=out) == EINVAL
     assert b"overlap" in _lib.lib().mllb_last_error()
+
+
+def test_sizes_whose_products_pass_64_bits():
+    L = _lib.lib()
+    assert L.mllb_beam_select_workspace(1 << 62, 4, 1000, 4) < 0
+    assert select(batch=1 << 62, done=None) == EINVAL
+    assert select(beam_stride=1 << 61) == EINVAL and select(batch_stride=1 << 61) == EINVAL
+    for batch, beams in ((1 << 62, 4), (4, 1 << 62), (1 << 32, 1 << 32)):
+        args = _lib.BeamRows(1 << 20, 2 << 20, 3 << 20, 4 << 20, batch, beams, 3)
+        assert L.mllb_beam_reorder(args, cache(), 5 << 20, 6 << 20, 7 << 20, 0, None) == EINVAL
+    assert L.mllb_paged_attention_workspace(2, 4, 2, 128, 1 << 62, 1 << 62) == _lib.MLLB_EUNSUPPORTED
+    assert attend(table_width=1 << 60) == EINVAL
+    assert attend(groups=1, prefix_table=4096, prefix_lens=4096, prefix_width=1 << 60) == EINVAL
+    assert attend(q_token_stride=1 << 62) == EINVAL
+    append = dict(qkv=1 << 20, tokens=3, positions=4096, rows=4096, page_table=4096, seqs=3, table_width=2, freqs=4096,
+                  rot_dim=128, q_heads=4, eps=1e-6, magnitude=1.0, q_out=1 << 30, qkv_stride=1 << 61)
+    assert L.mllb_paged_qkv_append(_lib.PagedAppend(**append), cache(), 0, None) == EINVAL
