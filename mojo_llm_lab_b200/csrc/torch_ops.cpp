@@ -129,8 +129,9 @@ mllb_paged_cache paged_cache(const at::Tensor& k, const at::Tensor& v, bool laye
   const int64_t lead = layers && k.dim() == 5 ? 1 : 0;
   if (type_of(k) != MLLB_TYPE_F16 && type_of(k) != MLLB_TYPE_BF16) refuse("k_cache must be torch.float16 or torch.bfloat16");
   need_view(k, "k_cache", 4 + lead);
-  if (v.scalar_type() != k.scalar_type() || v.sizes() != k.sizes() || v.strides() != k.strides())
-    refuse("v_cache must match k_cache in type, shape and strides");
+  bool match = v.scalar_type() == k.scalar_type() && v.sizes() == k.sizes();
+  for (int64_t i = 0; match && i < k.dim(); ++i) match = k.size(i) == 1 || v.stride(i) == k.stride(i);
+  if (!match) refuse("v_cache must match k_cache in type, shape and strides");
   const int64_t d = k.size(3 + lead);
   // A dimension of one element may carry any stride: it gets one that the kernels take.
   auto step = [&](int64_t dim) { return k.size(dim) > 1 ? k.stride(dim) : d * 8; };

@@ -209,3 +209,14 @@ def test_out_between_the_rows_of_q(tokens):
         mine.copy_(q)
         assert ops.paged_attention(mine, *args, q_start=ints([0, tokens]), out=out) is out
         assert torch.equal(out, want) and torch.equal(mine, q)
+
+
+def test_caches_of_one_head_with_other_strides():
+    """K by rows, V by heads: with one KV head the same layout, although torch gives other strides."""
+    table, pages, _ = P.tables([40, 3], 16, 6)
+    kc, vc = P.cache(pages, 1, 16, 64, F16, 7)
+    q = torch.randn(2, 4, 64, generator=torch.Generator().manual_seed(1)).to(F16).cuda()
+    k = kc.transpose(1, 2).contiguous().cuda().transpose(1, 2)
+    assert k.stride() != vc.stride()
+    out = ops.paged_attention(q, k, vc.cuda(), table.cuda(), ints([40, 3]))
+    assert torch.equal(out, ops.paged_attention(q, kc.cuda(), vc.cuda(), table.cuda(), ints([40, 3])))
