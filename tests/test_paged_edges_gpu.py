@@ -216,7 +216,8 @@ def test_caches_of_one_head_with_other_strides():
     table, pages, _ = P.tables([40, 3], 16, 6)
     kc, vc = P.cache(pages, 1, 16, 64, F16, 7)
     q = torch.randn(2, 4, 64, generator=torch.Generator().manual_seed(1)).to(F16).cuda()
-    k = kc.transpose(1, 2).contiguous().cuda().transpose(1, 2)
+    k = torch.empty(pages, 16, 1, 64, dtype=F16, device="cuda").transpose(1, 2)
+    k.copy_(kc)
     assert k.stride() != vc.stride()
     out = ops.paged_attention(q, k, vc.cuda(), table.cuda(), ints([40, 3]))
     assert torch.equal(out, ops.paged_attention(q, kc.cuda(), vc.cuda(), table.cuda(), ints([40, 3])))
