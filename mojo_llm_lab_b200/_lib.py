@@ -186,7 +186,7 @@ def native():
         lib()
         with _lock:
             if _native is None:
-                if not _build.TORCH_EXT.exists():
+                if not _build.torch_ext_current():
                     _build.build()
                 spec = importlib.util.spec_from_file_location("mllb200_torch", _build.TORCH_EXT)
                 module = importlib.util.module_from_spec(spec)

@@ -13,13 +13,15 @@
 
 * lib/mllb200_torch.so      -- Python extension: tensor checks and calls of the
                               paged-cache operators (csrc/torch_ops.cpp, host
-                              code only)
+                              code only, C++20); built last, and not where there
+                              is no torch
 
 The CUDA ones target `-gencode arch=compute_100a,code=sm_100a` only (B200).  The build
 is incremental on source mtimes; `python -m mojo_llm_lab_b200.build` forces it.
 """
 from __future__ import annotations
 
+import importlib.metadata
 import os
 import shutil
 import subprocess
@@ -60,6 +62,24 @@ def _stale(target: Path) -> bool:
     return target.stat().st_mtime < newest
 
 
+def _torch_stamp() -> str | None:
+    """What the extension module depends on besides its sources; None without torch."""
+    try:
+        return f"torch {importlib.metadata.version('torch')}, Python {sys.version}"
+    except importlib.metadata.PackageNotFoundError:
+        return None
+
+
+def _torch_stamp_file() -> Path:
+    return TORCH_EXT.with_suffix(".stamp")
+
+
+def torch_ext_current() -> bool:
+    """Whether the extension module is there and was built for this torch and this Python."""
+    file = _torch_stamp_file()
+    return TORCH_EXT.exists() and file.exists() and file.read_text() == _torch_stamp()
+
+
 def _run(cmd: list[str], log: Path, verbose: bool) -> None:
     env = dict(os.environ)
     # nvcc picks its host compiler from PATH; a CC/CXX override pointing at a
@@ -71,7 +91,7 @@ def _run(cmd: list[str], log: Path, verbose: bool) -> None:
     if verbose:
         sys.stderr.write(proc.stderr)
     if proc.returncode != 0:
-        raise RuntimeError(f"nvcc failed ({proc.returncode}):\n{proc.stderr[-4000:]}")
+        raise RuntimeError(f"{Path(cmd[0]).name} failed ({proc.returncode}):\n{proc.stderr[-4000:]}")
 
 
 def build(force: bool = False, verbose: bool = False) -> dict:
@@ -91,20 +111,6 @@ def build(force: bool = False, verbose: bool = False) -> dict:
               "-Wl,-rpath,$ORIGIN"], LIBDIR / "build_interpose.log", verbose)
         tmp.replace(INTERPOSE)
         built["interpose"] = str(INTERPOSE)
-    if force or _stale(TORCH_EXT) or TORCH_EXT.stat().st_mtime < LIB.stat().st_mtime:
-        import torch
-        torch_dir = Path(torch.__file__).resolve().parent
-        tmp = TORCH_EXT.with_suffix(".so.tmp")
-        cuda_inc = Path(nvcc()).resolve().parent.parent / "include"
-        system = [torch_dir / "include", torch_dir / "include" / "torch" / "csrc" / "api" / "include", cuda_inc,
-                  sysconfig.get_paths()["include"]]
-        _run([shutil.which("g++") or "g++", "-O2", "-std=c++20", "-fPIC", "-shared", "-Wall", f"-I{INCLUDE}",
-              *(arg for p in system for arg in ("-isystem", str(p))),
-              f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-o", str(tmp),
-              str(CSRC / "torch_ops.cpp"), f"-L{LIBDIR}", "-lmllb200", f"-L{torch_dir / 'lib'}", "-ltorch_python",
-              "-ltorch_cpu", "-lc10", "-lc10_cuda", "-Wl,-rpath,$ORIGIN"], LIBDIR / "build_torch.log", verbose)
-        tmp.replace(TORCH_EXT)
-        built["torch"] = str(TORCH_EXT)
     if force or _stale(HARNESS) or HARNESS.stat().st_mtime < LIB.stat().st_mtime:
         tmp = HARNESS.with_suffix(".tmp")
         _run([nvcc(), "-O2", "-std=c++17", f"-I{INCLUDE}", "-o", str(tmp), str(CSRC / "harness.cpp"),
@@ -118,6 +124,22 @@ def build(force: bool = False, verbose: bool = False) -> dict:
              LIBDIR / "build_cubin.log", verbose)
         tmp.replace(CUBIN)
         built["cubin"] = str(CUBIN)
+    stamp = _torch_stamp()
+    if stamp and (force or _stale(TORCH_EXT) or TORCH_EXT.stat().st_mtime < LIB.stat().st_mtime or not torch_ext_current()):
+        import torch
+        torch_dir = Path(torch.__file__).resolve().parent
+        tmp = TORCH_EXT.with_suffix(".so.tmp")
+        cuda_inc = Path(nvcc()).resolve().parent.parent / "include"
+        system = [torch_dir / "include", torch_dir / "include" / "torch" / "csrc" / "api" / "include", cuda_inc,
+                  sysconfig.get_paths()["include"]]
+        _run([shutil.which("g++") or "g++", "-O2", "-std=c++20", "-fPIC", "-shared", "-Wall", f"-I{INCLUDE}",
+              *(arg for p in system for arg in ("-isystem", str(p))),
+              f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-o", str(tmp),
+              str(CSRC / "torch_ops.cpp"), f"-L{LIBDIR}", "-lmllb200", f"-L{torch_dir / 'lib'}", "-ltorch_python",
+              "-ltorch_cpu", "-lc10", "-lc10_cuda", "-Wl,-rpath,$ORIGIN"], LIBDIR / "build_torch.log", verbose)
+        tmp.replace(TORCH_EXT)
+        _torch_stamp_file().write_text(stamp)
+        built["torch"] = str(TORCH_EXT)
     return built
 
 
