@@ -604,6 +604,8 @@ typedef struct mllb_paged_attn {
 } mllb_paged_attn;
 int64_t mllb_paged_attention_workspace(int64_t tokens, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
                                        int64_t seqs, int64_t groups);
+/* What this call takes of that, by its sizes and its tables' widths (pointers are not read). */
+int64_t mllb_paged_attention_call_workspace(const mllb_paged_attn *args, const mllb_paged_cache *cache);
 int mllb_paged_attention(const mllb_paged_attn *args, const mllb_paged_cache *cache, void *workspace,
                          int64_t workspace_bytes, unsigned flags, void *stream);
 

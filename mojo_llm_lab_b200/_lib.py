@@ -138,6 +138,7 @@ SIGNATURES = {
     "mllb_q4k_matmul_tokens": (C.c_int, [_P, _P, _P, _I64, _I64, _I64, _P, _I64, C.c_uint, _P]),
     "mllb_paged_qkv_append": (C.c_int, [C.POINTER(PagedAppend), C.POINTER(PagedCache), C.c_uint, _P]),
     "mllb_paged_attention_workspace": (_I64, [_I64, _I64, _I64, _I64, _I64, _I64]),
+    "mllb_paged_attention_call_workspace": (_I64, [C.POINTER(PagedAttn), C.POINTER(PagedCache)]),
     "mllb_paged_attention": (C.c_int, [C.POINTER(PagedAttn), C.POINTER(PagedCache), _P, _I64, C.c_uint, _P]),
     "mllb_beam_select_workspace": (_I64, [_I64, _I64, _I64, _I64]),
     "mllb_beam_select": (C.c_int, [C.POINTER(BeamScores), _P, _P, _P, _P, _I64, C.c_uint, _P]),

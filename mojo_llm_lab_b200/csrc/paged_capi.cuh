@@ -282,6 +282,16 @@ int check_attn_sizes(int64_t tokens, int64_t q_heads, int64_t kv_heads, int64_t 
   return MLLB_OK;
 }
 
+// What the plan of a call goes by.
+int check_attn_call(const mllb_paged_attn* p, const mllb_paged_cache* cache) {
+  const int rc = check_attn_sizes(p->tokens, p->q_heads, cache->kv_heads, cache->head_dim, p->seqs, p->groups);
+  if (rc) return rc;
+  if (p->table_width <= 0 || (p->groups && p->prefix_width <= 0)) return fail(MLLB_EINVAL, "page tables need a width");
+  if (p->table_width >= (1 << 30) / cache->page_size || (p->groups && p->prefix_width >= (1 << 30) / cache->page_size))
+    return fail(MLLB_EINVAL, "page tables of 2^30 rows or more");
+  return MLLB_OK;
+}
+
 template <int D, int R>
 int launch_few(const mllb::AttnArgs& a, const mllb::AttnPass& pass, const CUtensorMap& k, const CUtensorMap& v, bool bf16,
                int dev, cudaStream_t stream) {
@@ -466,6 +476,18 @@ int64_t mllb_paged_attention_workspace(int64_t tokens, int64_t q_heads, int64_t 
   return most;
 }
 
+int64_t mllb_paged_attention_call_workspace(const mllb_paged_attn* p, const mllb_paged_cache* cache) {
+  if (!p) return fail(MLLB_EINVAL, "null pointer");
+  mllb::PagedCache c;
+  PagedPlan plan;
+  int dev, rc;
+  if ((rc = paged_cache(cache, &c)) || (rc = check_attn_call(p, cache)) || (rc = current_device(&dev)) ||
+      (rc = paged_plan(p->tokens, p->q_heads, cache->kv_heads, cache->head_dim, p->seqs, p->groups, plan_choice(p, cache), dev,
+                       &plan)))
+    return rc;
+  return plan.bytes;
+}
+
 int mllb_paged_attention(const mllb_paged_attn* p, const mllb_paged_cache* cache, void* workspace, int64_t workspace_bytes,
                          unsigned flags, void* stream) {
   if (!p || !p->q || !p->out || !p->page_table || !p->seq_lens || !workspace) return fail(MLLB_EINVAL, "null pointer");
@@ -474,13 +496,10 @@ int mllb_paged_attention(const mllb_paged_attn* p, const mllb_paged_cache* cache
   int rc = paged_cache(cache, &c);
   if (rc) return rc;
   if (cache->layers != 1) return fail(MLLB_EINVAL, "attention takes one layer's cache");
-  if ((rc = check_attn_sizes(p->tokens, p->q_heads, cache->kv_heads, cache->head_dim, p->seqs, p->groups))) return rc;
+  if ((rc = check_attn_call(p, cache))) return rc;
   if (p->groups && (!p->prefix_table || !p->prefix_lens)) return fail(MLLB_EINVAL, "null pointer: prefix table or lengths");
   if (p->groups > 1 && !p->group_start) return fail(MLLB_EINVAL, "null pointer: group_start (needed for several groups)");
   if (!p->q_start && p->tokens != p->seqs) return fail(MLLB_EINVAL, "without q_start every sequence has one token");
-  if (p->table_width <= 0 || (p->groups && p->prefix_width <= 0)) return fail(MLLB_EINVAL, "page tables need a width");
-  if (p->table_width >= (1 << 30) / cache->page_size || (p->groups && p->prefix_width >= (1 << 30) / cache->page_size))
-    return fail(MLLB_EINVAL, "page tables of 2^30 rows or more");
   if (!(p->scale == p->scale) || p->scale - p->scale != 0.0) return fail(MLLB_EINVAL, "scale must be finite");
   const int64_t strides[4] = {p->q_token_stride, p->q_head_stride, p->out_token_stride, p->out_head_stride};
   for (int64_t s : strides)

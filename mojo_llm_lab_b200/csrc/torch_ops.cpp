@@ -266,11 +266,6 @@ PyObject* paged_attention(Args o) {
                                       &workspace});
   const c10::cuda::CUDAGuard guard(dev);
   if (!out.defined()) out = empty({tokens, q_heads, d}, q.scalar_type(), dev);
-  if (!workspace.defined()) {
-    const int64_t need = mllb_paged_attention_workspace(tokens, q_heads, cache.kv_heads, d, seqs, groups);
-    check(need, "paged_attention");
-    workspace = empty({need}, at::kByte, dev);
-  }
   // The stride of a dimension of one element counts as whole heads.
   auto step = [d](const at::Tensor& t, int64_t dim) { return t.size(dim) > 1 ? t.stride(dim) : d; };
   mllb_paged_attn a = {};
@@ -293,6 +288,11 @@ PyObject* paged_attention(Args o) {
   a.prefix_width = prefix_width;
   a.q_start = ptr<const int32_t>(q_start);
   a.scale = o[9] == Py_None ? 1.0 / std::sqrt(static_cast<double>(d)) : real(o[9]);
+  if (!workspace.defined()) {
+    const int64_t need = mllb_paged_attention_call_workspace(&a, &cache);
+    check(need, "paged_attention");
+    workspace = empty({need}, at::kByte, dev);
+  }
   const unsigned flags = truth(o[12]) ? MLLB_LAUNCH_PDL : 0;
   void* stream = stream_of(dev);
   check(unlocked([&] { return mllb_paged_attention(&a, &cache, workspace.data_ptr(), workspace.numel(), flags, stream); }),

@@ -221,3 +221,26 @@ def test_caches_of_one_head_with_other_strides():
     assert k.stride() != vc.stride()
     out = ops.paged_attention(q, k, vc.cuda(), table.cuda(), ints([40, 3]))
     assert torch.equal(out, ops.paged_attention(q, kc.cuda(), vc.cuda(), table.cuda(), ints([40, 3])))
+
+
+# ------------------------------------------------------------------ memory
+
+@pytest.mark.parametrize("seqs,tokens,prefix,most", [(512, 10, 40, 44), (1024, 12, 40, 44), (512, 1, 0, 8), (64, 1, 30, 8)])
+def test_attention_allocates_for_the_plan_that_it_takes(seqs, tokens, prefix, most):
+    """32 query and 8 KV heads of 128: MB beside the result.  Two segments of 256 rows a CTA take 39 MB, with up to 64 rows
+    a tile and two CTAs an SM 20, with 16 rows 5."""
+    page, hq, hk, d = 16, 32, 8, 128
+    table = torch.zeros(seqs, 2, dtype=torch.int32).cuda()
+    kc, vc = (x.cuda() for x in P.cache(4, hk, page, d, F16, 5))
+    q = torch.zeros(seqs * tokens, hq, d, dtype=F16, device="cuda")
+    more = {}
+    if prefix:
+        more = dict(prefix_table=torch.zeros(1, -(-prefix // page), dtype=torch.int32).cuda(), prefix_lens=ints([prefix]))
+    if tokens > 1:
+        more["q_start"] = ints([tokens * i for i in range(seqs + 1)])
+    lens, out = ints([20] * seqs), torch.empty_like(q)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    ops.paged_attention(q, kc, vc, table, lens, out=out, **more)
+    assert torch.cuda.max_memory_allocated() - before <= most * 2 ** 20

@@ -98,3 +98,12 @@ def test_sizes_whose_products_pass_64_bits():
     append = dict(qkv=1 << 20, tokens=3, positions=4096, rows=4096, page_table=4096, seqs=3, table_width=2, freqs=4096,
                   rot_dim=128, q_heads=4, eps=1e-6, magnitude=1.0, q_out=1 << 30, qkv_stride=1 << 61)
     assert L.mllb_paged_qkv_append(_lib.PagedAppend(**append), cache(), 0, None) == EINVAL
+
+
+def test_call_workspace_refuses_what_the_call_refuses():
+    need = _lib.lib().mllb_paged_attention_call_workspace
+    assert need(None, cache()) == EINVAL and need(_lib.PagedAttn(), None) == EINVAL
+    sizes = dict(tokens=3, q_heads=4, seqs=3, table_width=2)
+    assert need(_lib.PagedAttn(**{**sizes, "tokens": 0}), cache()) == EINVAL
+    assert need(_lib.PagedAttn(**{**sizes, "table_width": 1 << 60}), cache()) == EINVAL
+    assert need(_lib.PagedAttn(**sizes), cache(head_dim=96)) == _lib.MLLB_EUNSUPPORTED
