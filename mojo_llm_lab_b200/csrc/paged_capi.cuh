@@ -510,6 +510,8 @@ int mllb_paged_attention(const mllb_paged_attn* p, const mllb_paged_cache* cache
     return fail(MLLB_EINVAL, "rows of out overlap");
   if (!aligned(p->q, 16) || !aligned(p->out, 16) || !aligned(workspace, 16))
     return fail(MLLB_EALIGN, "q, out and workspace must be 16-byte aligned");
+  for (const int32_t* at : {p->page_table, p->seq_lens, p->prefix_table, p->prefix_lens, p->group_start, p->q_start})
+    if (at && !aligned(at, 4)) return fail(MLLB_EALIGN, "tables, lengths and starts must be 4-byte aligned");
   const bool in_place = p->q == p->out && (p->tokens == 1 || p->q_token_stride == p->out_token_stride) &&
                         (p->q_heads == 1 || p->q_head_stride == p->out_head_stride);
   if (!in_place && out_overlaps_q(p, cache->head_dim))

@@ -107,3 +107,10 @@ def test_call_workspace_refuses_what_the_call_refuses():
     assert need(_lib.PagedAttn(**{**sizes, "tokens": 0}), cache()) == EINVAL
     assert need(_lib.PagedAttn(**{**sizes, "table_width": 1 << 60}), cache()) == EINVAL
     assert need(_lib.PagedAttn(**sizes), cache(head_dim=96)) == _lib.MLLB_EUNSUPPORTED
+
+
+@pytest.mark.parametrize("name", ["page_table", "seq_lens", "prefix_table", "prefix_lens", "group_start", "q_start"])
+def test_attention_indices_off_their_alignment(name):
+    """A misaligned 4-byte load would end the context."""
+    more = dict(groups=1, prefix_table=4096, prefix_lens=4096, prefix_width=2, group_start=4096, q_start=4096)
+    assert attend(**{**more, name: 4098}) == _lib.MLLB_EALIGN
