@@ -536,7 +536,7 @@ int mllb_paged_attention(const mllb_paged_attn* p, const mllb_paged_cache* cache
   a.lens = p->seq_lens;
   a.prefix_table = p->prefix_table;
   a.prefix_lens = p->prefix_lens;
-  a.group_start = p->group_start;
+  a.group_start = p->groups ? p->group_start : nullptr;
   a.q_start = p->q_start;
   a.width = static_cast<int>(p->table_width);
   a.prefix_width = static_cast<int>(p->groups ? p->prefix_width : 0);

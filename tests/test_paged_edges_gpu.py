@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import paged_util as P
-from mojo_llm_lab_b200 import ops
+from mojo_llm_lab_b200 import _lib, ops
 
 pytestmark = pytest.mark.gpu
 
@@ -244,3 +244,19 @@ def test_attention_allocates_for_the_plan_that_it_takes(seqs, tokens, prefix, mo
     before = torch.cuda.memory_allocated()
     ops.paged_attention(q, kc, vc, table, lens, out=out, **more)
     assert torch.cuda.max_memory_allocated() - before <= most * 2 ** 20
+
+
+def test_group_starts_without_groups_are_not_read():
+    """The C entry with groups 0 and a group_start all the same."""
+    table, pages, _ = P.tables([40, 3], 16, 6)
+    kc, vc = (x.cuda() for x in P.cache(pages, 2, 16, 64, F16, 7))
+    q = torch.randn(2, 4, 64, generator=torch.Generator().manual_seed(1)).to(F16).cuda()
+    table, lens, starts = table.cuda(), ints([40, 3]), ints([10 ** 6])
+    want, out = ops.paged_attention(q, kc, vc, table, lens), torch.empty_like(q)
+    cache = _lib.PagedCache(kc.data_ptr(), vc.data_ptr(), pages, 2, 16, 64, *kc.stride()[:3], 1, 0, _lib.TYPE_F16)
+    call = _lib.PagedAttn(q.data_ptr(), out.data_ptr(), 2, 4, 256, 64, 256, 64, table.data_ptr(), lens.data_ptr(), 2,
+                          table.shape[1], None, None, starts.data_ptr(), 0, 0, None, 0.125)
+    work = torch.empty(_lib.lib().mllb_paged_attention_call_workspace(call, cache), dtype=torch.uint8, device="cuda")
+    _lib.check(_lib.lib().mllb_paged_attention(call, cache, work.data_ptr(), work.numel(), 0,
+                                               torch.cuda.current_stream().cuda_stream), "attention")
+    assert torch.equal(out, want) and ops.device_error() == 0
