@@ -967,7 +967,9 @@ __global__ void __launch_bounds__(256)
     seq = lo;
   }
   AttnJoin<D> join;
-  const bool done = first.plan[first.entities] && (first.mode == kAttnBoth || second.plan[second.entities]);
+  // Loaded beside the parts, looked at before the store.
+  const bool two = first.mode != kAttnBoth;
+  const int done = first.plan[first.entities], done_own = two ? second.plan[second.entities] : 1;
   if (there) {
     const int g = attn_group_of(a, seq);
     AttnRowParts pre = {0, -1, 0, 0};
@@ -981,7 +983,7 @@ __global__ void __launch_bounds__(256)
                                  : attn_slot<D>(own_pass, own.c0 + i - shared_segments + own.item, own.row);
     });
   }
-  if (!join.gather(shared, warp, lane, part, parts) || !there || !done) return;
+  if (!join.gather(shared, warp, lane, part, parts) || !there || !(done & done_own)) return;
   attn_store_row<D, kBf16>(a, token, head, lane, join.sum, join.acc);
 }
 
