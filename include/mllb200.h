@@ -576,19 +576,26 @@ int mllb_paged_qkv_append(const mllb_paged_append *args, const mllb_paged_cache 
  * Sequence b's tokens are q_start[b] .. q_start[b + 1] - 1 (q_start NULL: one
  * each), its last ones: of n tokens, token i sees its own rows below
  * seq_lens[b] - n + i + 1.  Sequences group_start[g] .. group_start[g + 1] - 1
- * also see all prefix_lens[g] rows of prefix_table[g]; a group's prefix is
- * read once for all its sequences where they have few tokens.  groups 0: no
- * prefixes; group_start NULL: one group of all sequences.  A token that sees
+ * also see all prefix_lens[g] rows of prefix_table[g].  A group's prefix is read
+ * once for all its sequences where they have few tokens and the prefix is long,
+ * otherwise by each sequence again (from L2 as a rule); that goes by the tokens'
+ * mean and by the tables' widths, which the host sees, not by the lengths: a
+ * short prefix in a table of the largest context costs up to twice as much as in
+ * a narrow one.  groups 0: no prefixes; group_start NULL: one group of all sequences.  A token that sees
  * nothing gets zeros; tokens behind q_start[seqs] stay as they are.  q_start and
  * group_start ascend within [0, tokens] and [0, seqs]: what lies outside counts
  * as the end, where they descend out is of no use, both set bit 8.  Rows
  * behind a sequence's length may hold anything, NaN too; the visible ones,
  * and those of a sequence's later tokens, must be finite.  q head h reads KV
  * head h / (q_heads / kv_heads).  q and out have the cache's type, and out
- * may be q itself (with its strides) but share no other rows with it; fp32 softmax and sums, the weights rounded to the cache's
- * type for the products with V.  workspace: mllb_paged_attention_workspace bytes (the number
- * depends on the current device), 16-byte aligned, any contents; calls that
- * share it must not overlap on the GPU.  seqs + groups <= 2048.
+ * may be q itself (with its strides) but share no other rows with it.  Softmax
+ * and sums are fp32, the weights rounded to the cache's type for the products
+ * with V: half a step each, in fp16 from 2^-21 of a row's largest weight on, and
+ * 2^-32 of the largest below.  workspace: mllb_paged_attention_workspace bytes,
+ * enough for tables of any width (the number depends on the current device), or
+ * what mllb_paged_attention_call_workspace gives for the call; 16-byte aligned,
+ * any contents; calls that share it must not overlap on the GPU.
+ * seqs + groups <= 2048.
  */
 typedef struct mllb_paged_attn {
     const void *q;
@@ -604,7 +611,7 @@ typedef struct mllb_paged_attn {
 } mllb_paged_attn;
 int64_t mllb_paged_attention_workspace(int64_t tokens, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
                                        int64_t seqs, int64_t groups);
-/* What this call takes of that, by its sizes and its tables' widths (pointers are not read). */
+/* What one call needs, by its sizes and its tables' widths; nothing is read through its pointers. */
 int64_t mllb_paged_attention_call_workspace(const mllb_paged_attn *args, const mllb_paged_cache *cache);
 int mllb_paged_attention(const mllb_paged_attn *args, const mllb_paged_cache *cache, void *workspace,
                          int64_t workspace_bytes, unsigned flags, void *stream);
@@ -618,7 +625,10 @@ int mllb_paged_attention(const mllb_paged_attn *args, const mllb_paged_cache *ca
  * -inf, +inf as the largest finite fp32.  A logit of -inf is no candidate;
  * a done beam's only candidate is end_token at the beam's score.  Places
  * without a candidate: -inf, -1, -1.  beams and n at most 64, vocab at most
- * 2^26.  Scores are compared in fp64.  workspace as for the attention.  Results
+ * 2^26.  Scores are formed and compared in fp64, from log-sums whose terms are
+ * fp32 exponentials: each beam's may be off by 2^-20, so candidates of different
+ * beams that lie closer than 2^-19 may change places; in a beam the order is
+ * that of the logits.  workspace as for the attention.  Results
  * must not overlap one another, scores, done or the workspace, except that
  * out_scores may be scores where n is beams.
  */
@@ -643,8 +653,8 @@ int mllb_beam_select(const mllb_beam_scores *args, float *out_scores, int32_t *o
  * lowest r) keeps it and every other child gets fresh[r] in its place, with
  * the rows held copied for K and V of all layers; used[r] = 1 where fresh[r]
  * was taken.  fresh: distinct pages that no table line names.  A negative
- * parent ends the row (length 0, table -1, reserved pages too), one past the beams also sets
- * device error bit 9 (mask 0x200).  table_out, lens_out and used must not
+ * parent ends the row (length 0, table -1, reserved pages too), one past the
+ * beams also sets device error bit 9 (mask 0x200).  table_out, lens_out and used must not
  * overlap the inputs or one another.
  */
 typedef struct mllb_beam_rows {

@@ -5,7 +5,8 @@
 // best, fp64 scores of different logits meet), then to the lower token.  Within
 // a beam the order is that of the logits, so one pass over them finds both the n
 // best of every chunk and the chunk's part of the sum; a second, small kernel
-// joins them in fp64.
+// joins them in fp64.  The scan's exponentials are fp32 (ex2, and 16 terms at a
+// time): a log-sum may be off by 2^-20.
 //
 // Logits: NaN counts as -inf, +inf as the largest finite fp32, and -inf is
 // no candidate (nor is anything of a beam whose cum is -inf or NaN).
@@ -170,9 +171,10 @@ __device__ __forceinline__ void beam_best(BeamScratch& sh, int total, int n, uns
 // the maxima and read again, and the n best of their 16 n logits taken.
 // Groups are in the order of their logits, so ties come out right.
 // Key of a logit: its ordered bits above the complement of its index; 0 is no
-// candidate.  Bound: issue slots, about 8 a logit (unpack, NaN, maximum,
-// difference, product, ex2, sum), rather than its 2 or 4 bytes from HBM, and
-// for short chunks the latencies of the selection.  Both kernels, 32 x 8 rows of
+// candidate.  No unit is full (32 x 8 rows: issue slots 54 %, exponentials 39 %,
+// DRAM 23 %): about 8 slots a logit while the scan runs (unpack, NaN, maximum,
+// difference, product, ex2, sum), then the barriers of two selections, when most
+// warps wait; for short chunks those are all.  Both kernels, 32 x 8 rows of
 // 151936 in bf16: n = 8 33 us, n = 16 with some of the beams done 39; the
 // bytes alone 12.  4 rows in fp32: 11.
 template <int kType, bool kVector>

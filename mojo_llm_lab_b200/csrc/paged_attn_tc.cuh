@@ -21,7 +21,9 @@
 // outgrow it by 2^8: until then its weights are up to 2^8 instead of up to 1
 // (2^15 with fp16's lift of 7), which the 16-bit types hold as well and fp32
 // sums too.  After the first tiles O is hardly ever touched by the softmax
-// warps.
+// warps.  The price is that the largest weight is not 1, which has no rounding:
+// prompts in bf16 are 2.3e-3 off the exact values (rounding the result alone is
+// 1.7e-3), ragged sequences in the few-row kernel, whose maxima always move, 1.8e-3.
 //
 // Where an item ends, the next one's queries and first keys are on their way
 // already: warp 10 posts segments two ahead and lets TMA bring their queries
@@ -32,8 +34,11 @@
 // Bound: a key tile of 256 rows takes the tensor cores 2048 cycles and the
 // exponentials as many (16 a cycle), the rest of the softmax issue slots beside
 // them; the two streams hide less of one behind the other than they might, and
-// the clock falls under this load.  Prompts of 1 to 1024 tokens behind a prefix of 1500 rows
-// (119 GFLOP) take 131 us, 0.91 PFLOP/s, and one of 8000 tokens 451 us, 1.16.
+// the clock falls under this load.  4 prompts of up to 1024 tokens behind a
+// prefix of 1500 rows (119 GFLOP): 150 us on changing inputs, 0.79 PFLOP/s, 130
+// us replayed on one; one of 8000 tokens, replayed, 447 to 490 (it goes by the
+// clock), 1.07 to 1.17.  With heads of 128 the 168 registers do not quite do
+// (68 to 88 bytes of spill stores a thread).
 #pragma once
 
 #include "paged_attn.cuh"

@@ -175,11 +175,11 @@ enum : unsigned { kPlanRepeat = 1, kPlanLong = 2, kPlanChoices = 4 };
 
 // Row tile for entities of `rows` query rows: up to 64 the kernel for few rows
 // a key, in its narrowest shape that holds them; beyond, the tensor cores'.
-// 48 sequences of 4000 rows, 8 KV heads: 4 rows 101 us (in tiles of 32: 105), 32
-// rows 110 us (in tiles of 64: 168).  33 to 64 rows lie between, and the length
-// decides: 48 sequences of 16 tokens on 60 rows take the few-row kernel 19 us and
-// the other, whose items start and end dearer, 22; on 700 rows 53 and 48, on 4000
-// rows 172 and 133.
+// 48 sequences of 2000 to 4000 rows, 8 KV heads: 4 query rows 102 us (in tiles of
+// 32: 105), 32 109 us (in tiles of 64: 168).  33 to 64 lie between, and the length
+// decides: 48 sequences of 16 tokens on 30 to 60 rows take the few-row kernel 20 us
+// and the other, whose items start and end dearer, 22; on 350 to 700 rows 53 and
+// 48, on 2000 to 4000 172 and 134.
 int tile_rows(int64_t rows, bool longs) {
   return rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 && !longs ? 64 : mllb::AttnMany<128>::kRows;
 }
@@ -197,7 +197,9 @@ bool one_softmax(int64_t seq_rows, int64_t seqs, int64_t groups, bool repeat) {
 // against 19.5; of 4000, 236 MB, 32.4 against 22.7), 192 MB against a pass each
 // (40 of 1000, 156 MB, 28.0 against 31.8; of 4000, 614 MB, 63 against 37).
 // And whether a sequence's item is long by the same bound: 512 rows and more
-// (tile_rows).
+// (tile_rows).  The lengths are on the device, so tables far wider than they are
+// take the other plan: 22 sequences of 100 rows on a prefix of 30 14.4 us in
+// narrow tables, 29.7 in ones of 8192 rows; 111 of 20 on 74 20.3 and 36.1.
 unsigned plan_choice(const mllb_paged_attn* p, const mllb_paged_cache* c) {
   const int64_t prefix = p->groups ? p->prefix_width * c->page_size : 0, rows = p->tokens * (p->q_heads / c->kv_heads);
   const int64_t again = (p->seqs - p->groups) * prefix * c->kv_heads * c->head_dim * 4;
@@ -209,7 +211,9 @@ unsigned plan_choice(const mllb_paged_attn* p, const mllb_paged_cache* c) {
 }
 
 // Mean query rows (tokens x query heads of a KV head) of a sequence and of a
-// group decide the shape.  A sequence with a row tile's worth of rows shares
+// group decide the shape, for all sequences of the call: a prompt's chunk of 512
+// tokens on 8000 rows beside 128 single tokens takes 515 us, the two calls apart
+// 69 and 206.  A sequence with a row tile's worth of rows shares
 // nothing more by going through its group, so prefix and own rows then run as
 // one softmax (no segments to join); so they do where kPlanRepeat says.  Otherwise
 // the prefix runs once a group (16 sequences over a prefix of 8000 rows: up to 32

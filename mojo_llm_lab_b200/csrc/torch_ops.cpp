@@ -2,8 +2,9 @@
 // tensors, result allocation, the current stream, and the C ABI call.
 //
 // ops.py does this in Python for the other operators.  The single-token forms
-// here take 3-17 us on the GPU, with ten or more tensors each to check: in
-// Python that took 20-32 us a call, in this form 1-2 us beside the launches.
+// here take 3-17 us on the GPU, with ten or more tensors each to check: a call
+// took 20-32 us from Python in that form, in this one 4-10, launches and
+// allocations included.
 //
 // Every function takes the positional arguments of its namesake in ops.py.
 // Errors are those of ops.py: ValueError for shapes, types and alignment,

@@ -758,7 +758,8 @@ def paged_qkv_append(qkv: torch.Tensor, positions: torch.Tensor, rows: torch.Ten
 
 def paged_attention_workspace(tokens: int, q_heads: int, kv_heads: int, head_dim: int, seqs: int, groups: int,
                               device) -> torch.Tensor:
-    """Workspace for paged_attention (reusable by calls of these sizes that do not overlap on the GPU)."""
+    """Workspace for paged_attention, enough for tables of any width (reusable by calls of these sizes that do not overlap
+    on the GPU).  A call without one allocates only what its plan takes."""
     dev = torch.device(device)
     with torch.cuda.device(dev):
         need = int(lib().mllb_paged_attention_workspace(tokens, q_heads, kv_heads, head_dim, seqs, groups))
@@ -776,10 +777,12 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
 
     Sequence b's own rows are the first seq_lens[b] of its line of page_table; its tokens are q_start[b] ..
     q_start[b + 1] - 1 (None: one each), the last ones of those rows, each seeing the rows up to its own.  Sequences
-    group_start[g] .. group_start[g + 1] - 1 (None: all) see the prefix_lens[g] rows of prefix_table[g] too; these are
-    read once for all of a group's sequences.  A token that sees nothing gets zeros; tokens behind q_start[-1] are left
-    as they are.  What a row's mask hides may hold anything behind a sequence's length; rows that later tokens of the
-    sequence see must be finite.  At most 2048 sequences and groups.  scale: 1 / sqrt(head_dim) unless given.  out may
+    group_start[g] .. group_start[g + 1] - 1 (None: all) see the prefix_lens[g] rows of prefix_table[g] too.  A long
+    prefix of sequences with few tokens is read once for all of them, a short one by each again; what is long goes by the
+    tables' widths, which the host sees, so tables should be no wider than the longest context that they must reach.
+    A token that sees nothing gets zeros; tokens behind q_start[-1] are left as they are.  What a row's mask hides may hold anything behind a sequence's length; rows that later tokens of the
+    sequence see must be finite.  Softmax and sums are fp32, the weights rounded to the caches' type for the products
+    with V.  At most 2048 sequences and groups.  scale: 1 / sqrt(head_dim) unless given.  out may
     be q, or must share no rows with it."""
     return native().paged_attention(q, k_cache, v_cache, page_table, seq_lens, prefix_table, prefix_lens, group_start,
                                     q_start, scale, out, workspace, pdl)
@@ -789,7 +792,8 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, n: int | None = None
                 end_token: int = -1, out=None, workspace: torch.Tensor | None = None,
                 pdl: bool = False) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """The n (default: beams) best continuations of every batch entry by scores[b, w] + log_softmax(logits[b, w])[v]:
-    (scores fp32, tokens int32, parents int32), each [batch, n], best first, ties to the lower beam, then token.
+    (scores fp32, tokens int32, parents int32), each [batch, n], best first, ties to the lower beam, in it to the
+    larger logit, then to the lower token.  Scores are compared in fp64, from log-sums that may be off by 2^-20.
 
     logits [batch, beams, vocab] in fp32, fp16 or bf16, scores fp32 [batch, beams].  -inf logits are never chosen; a
     beam that is done (bool or uint8 [batch, beams]) offers only end_token at its score.  Places without a candidate
