@@ -35,9 +35,10 @@ bool meet(const Span& a, const Span& b) {
 
 // Whether two of the rows of d elements at t * token + h * head, t < tokens, h < heads, have an element in common.
 bool rows_overlap(int64_t tokens, int64_t token, int64_t heads, int64_t head, int64_t d) {
-  if (tokens > 1 && token < d) return true;
+  if ((tokens > 1 && token < d) || (heads > 1 && head < d)) return true;
+  if (tokens == 1 || heads == 1 || token >= (heads - 1) * head + d || head >= (tokens - 1) * token + d) return false;
   for (int64_t h = 1; h < heads; ++h) {  // row (0, h) lies between rows (t, 0) and (t + 1, 0), or behind all
-    const int64_t at = h * head, t = tokens > 1 ? at / token : 0, behind = at - t * token;
+    const int64_t at = h * head, t = at / token, behind = at - t * token;
     if ((t < tokens && behind < d) || (t + 1 < tokens && token - behind < d)) return true;
   }
   return false;
