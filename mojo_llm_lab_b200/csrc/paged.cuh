@@ -260,8 +260,8 @@ constexpr int kReorderAhead = 8;
 // the first CTA writes them.  Columns behind stay the row's own, pages that its
 // caller reserved ahead: the parent's would be every child's, who would write
 // over one another.  Where the row's own rows were is no such page (a sibling may
-// hold it), so those columns become -1.  A page that is part full goes on being written by its
-// beam, so only the first child of a parent keeps it: the others take
+// hold it), so those columns become -1.  A page that is part full goes on being
+// written by its beam, so only the first child of a parent keeps it: the others take
 // fresh[row], and the CTAs copy the rows held so far, one (layer, K or V,
 // head) a warp, 16 bytes a lane.  Bound: HBM where there is much to copy, as
 // many bytes in as out (16 x 8 beams, 36 layers of 8 heads, 13 rows of a page:

@@ -59,9 +59,9 @@ struct AttnPass {
   int slots;       // capacity of the workspace
   int rows, keys;  // R and KT of the kernel that ran it (for the merge)
   // For the kernel that joins.  dense: [entities] items before each entity, 1
-  // (0: the starts descend, nothing was done), then int2 [items] first and last CTA of an item; otherwise AttnCut, the
-  // number of records first (as segments), then one an item (by_item: there are
-  // no more items than CTAs) or one a CTA.
+  // (0: the starts descend, nothing was done), then int2 [items] first and last
+  // CTA of an item; otherwise AttnCut, the number of records first (as segments),
+  // then one an item (by_item: there are no more items than CTAs) or one a CTA.
   int32_t* plan;
   int by_item;
   float* acc;      // [slots][R][D]

@@ -441,7 +441,9 @@ __global__ void __launch_bounds__(384, 1)
     bool more = take_own(&s);
     if (more) row = load_queries(s);
     while (more && !stuck) {
-      float top = -INFINITY, sum = 0.0f;
+      // Rows that do not exist are other tokens' (being written, where out is q):
+      // nothing outgrows their maximum, so they have no say in when the warp's move.
+      float top = row.token >= 0 ? -INFINITY : INFINITY, sum = 0.0f;
       for (int k = s.begin; k < s.end; ++k, ++sn) {
         const AttnTile tile = attn_tile<KT>(s.ent, k);
         const int held = tile.rows - tile.row0;
@@ -477,9 +479,7 @@ __global__ void __launch_bounds__(384, 1)
 #pragma unroll
         for (int i = 0; i < 4; ++i) mc[i] = fmaxf(mc[i], x[KT - 4 + i]);
         const float m = fmaxf(fmaxf(mc[0], mc[1]), fmaxf(mc[2], mc[3])) * scale;
-        // Rows that do not exist are other tokens' (being written, where out is
-        // q): they have no say in when the warp's maxima move.
-        if (__any_sync(0xffffffffu, m > top + 8.0f && row.token >= 0)) {
+        if (__any_sync(0xffffffffu, m > top + 8.0f)) {
           const float z = fmaxf(m, top), f = z == -INFINITY ? 0.0f : ex2(top - z);
           top = z;
           sum *= f;
