@@ -38,7 +38,7 @@
 // prefix of 1500 rows (119 GFLOP): 150 us on changing inputs, 0.79 PFLOP/s, 130
 // us replayed on one; one of 8000 tokens, replayed, 447 to 490 (it goes by the
 // clock), 1.07 to 1.17.  With heads of 128 the 168 registers do not quite do
-// (68 to 88 bytes of spill stores a thread).
+// (52 to 56 bytes of spill stores a thread).
 #pragma once
 
 #include "paged_attn.cuh"
